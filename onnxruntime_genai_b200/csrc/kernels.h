@@ -340,6 +340,21 @@ int ogb_paged_attention_kv8(const void* q, int q_stride, const void* k_cache, co
                         int max_q_len, int Hq, int Hkv, int D, int splits, int kv_chunk, void* scratch, long long scratch_bytes,
                         int cache_slots, const int32_t* order, int* status, void* stream);
 
+// ---- quantize_fp4.cu, linear_fp4.cu (4-bit floating-point rows and weights in the layout of fp4_matrix.cuh; form 0: nvfp4, 1: mxfp4)
+long long ogb_fp4_matrix_bytes(int rows, int K, int form);      // of one buffer of codes, block scales and row scales; -1: refused
+int ogb_quantize_fp4(const void* x, long long ldx, int x_fp32, int rows, int K, int form, void* data, void* stream);
+int ogb_dequantize_fp4(const void* data, int rows, int K, int form, void* out, long long ldo, int out_fp32, void* stream);
+// x != null: these rows are quantised into a_data first; null: a_data holds quantised rows.  pair: silu(gate) * up of blocks of 64 + 64 weight rows
+int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T, const void* w_data, int N, int K, int form, void* out, long long ldc,
+                   int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, void* stream);
+
+// ---- moe_few.cu (a whole expert layer for up to eight tokens; rule: mode of ogb_moe_topk; weights 0: bf16, 1 / 2: packed MXFP4 in its fp16 / bf16 form;
+// act 1: silu(gate) * up, 2: clamped SwiGLU; gate_up in blocks of 64 gate + 64 up rows)
+long long ogb_moe_few_scratch_bytes(int T, int top, int I);     // -1: refused
+int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b, const void* down,
+                       const void* down_b, void* out, int T, int H, int I, int E, int top, int rule, int weights, int act, float alpha, float limit,
+                       void* scratch, void* stream);
+
 // ---- sampling.cu
 int ogb_sample(const float* logits, long long row_stride, int rows, int vocab, const int32_t* top_k, const float* top_p,
                const float* temperature, const unsigned long long* seeds, const int32_t* positions, int32_t* out, void* stream);

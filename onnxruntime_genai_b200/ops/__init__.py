@@ -15,7 +15,9 @@ import torch
 
 from . import reference as ref
 from . import _lib
+from . import fp4_matrix
 from .fp4 import Fp4Experts
+from .fp4_matrix import Fp4Matrix
 from .w4 import QuantizedEmbedding, W4Weight, unpack_ort_q4
 
 _ACT = {"silu": 0, "gelu": 1, "gelu_tanh": 1, "relu": 2, "gelu_erf": 3, "relu2": 4}
@@ -381,7 +383,17 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     norm_eps > 0: an RMS norm folded into the GEMM - x holds the un-normalised rows, w already carries the norm's weight
     (w * norm_weight along K), and row m of the product is scaled by rsqrt(mean(x[m]^2) + norm_eps).
     splits: 0 leaves the kernel to the launcher; n > 0 asks for the one that cuts k in n parts, n < 0 for the one on pairs of SMs with -n token
-    tiles where it can take the product (no reduction over ranks, no folded norm)."""
+    tiles where it can take the product (no reduction over ranks, no folded norm).
+    w an Fp4Matrix: x (bf16 or fp32 rows, or an Fp4Matrix of the same form) is quantised to 4 bits too, and the block-scaled tensor-core product takes both
+    as they are; splits is not looked at."""
+    if isinstance(w, Fp4Matrix):
+        if all_reduce or reduce_scatter is not None:
+            raise RuntimeError("products of 4-bit floating-point weights are not reduced over ranks")
+        if norm_eps > 0:
+            if isinstance(x, Fp4Matrix):
+                raise ValueError("a norm cannot be folded into rows that are quantised already")
+            x = rms_scale(x, norm_eps)
+        return _linear_fp4(x, w, bias, residual, out_fp32, out)
     if isinstance(w, W4Weight):
         if norm_eps > 0:
             x = rms_scale(x, norm_eps)
@@ -421,6 +433,84 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     if residual is not None and residual.dtype == torch.float32:
         flags |= GEMM_FP32_RESIDUAL       # an fp32 residual stream, updated in place by the epilogue when `out` is the residual itself
     return _gemm(x, w, out, bias, residual, flags, splits, fused)
+
+
+def _on(device):
+    """The stream that a call on `device` uses: the current one of that device, made the current device for the call where it is another."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def quantize_fp4(x, form: str = "nvfp4") -> Fp4Matrix:
+    """Rows [T, K] (bf16 or fp32) as 4-bit floating-point numbers in blocks along K.
+    "nvfp4": blocks of 16 with an e4m3 scale, a power of two per row; "mxfp4": blocks of 32 with a power of two.  Codes are the nearest ones, ties to the
+    even code (csrc/quantize_fp4.cu gives the rules).  A row that holds an infinity or a NaN reads back, and multiplies, as NaN throughout.
+    The result serves as the rows of `linear` and `gate_up_act` with weights of the same form, so that several products share one quantisation."""
+    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"quantize_fp4 takes rows [T, K] in bfloat16 or float32, not {tuple(x.shape)} in {x.dtype}")
+    T, K = x.shape
+    Fp4Matrix.check(T, K, form)
+    if not x.is_cuda:
+        return fp4_matrix.quantize(x, form)
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    data = torch.empty(fp4_matrix.matrix_bytes(T, K, form), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _lib.check(_lib.lib().ogb_quantize_fp4(x.data_ptr(), x.stride(0), int(x.dtype == torch.float32), T, K, fp4_matrix.FORMS[form], data.data_ptr(),
+                                               _stream()), "quantize_fp4")
+    return Fp4Matrix(data, T, K, form)
+
+
+def _dequantize_fp4(m: Fp4Matrix, dtype):
+    out = torch.empty(m.rows, m.K, dtype=dtype, device=m.device)
+    with _on(m.device):
+        _lib.check(_lib.lib().ogb_dequantize_fp4(m.data.data_ptr(), m.rows, m.K, fp4_matrix.FORMS[m.form], out.data_ptr(), m.K, int(dtype == torch.float32),
+                                                 _stream()), "dequantize_fp4")
+    return out
+
+
+def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=None, pair=False):
+    """The product of 4-bit rows and weights; x: rows still to be quantised, or an Fp4Matrix of w's form."""
+    N, K = w.shape
+    n_out = N // 2 if pair else N
+    given = isinstance(x, Fp4Matrix)
+    if given and x.form != w.form:
+        raise ValueError(f"rows in {x.form} and weights in {w.form}")
+    if not given and (x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32)):
+        raise ValueError(f"rows [T, K] in bfloat16 or float32 are wanted, not {tuple(x.shape)} in {x.dtype}")
+    T = x.shape[0]
+    if x.shape[1] != K:
+        raise ValueError(f"rows of {x.shape[1]} and weights of {K}")
+    if x.device != w.device or any(t is not None and t.device != w.device for t in (bias, residual, out)):
+        raise ValueError("rows, weights, bias, residual and output are on different devices")
+    if bias is not None and (bias.shape != (N,) or (w.is_cuda and (bias.dtype != torch.bfloat16 or bias.stride(0) != 1))):
+        raise ValueError(f"the bias of {N} outputs is bfloat16 [{N}]")
+    if residual is not None and (residual.shape != (T, n_out) or (w.is_cuda and (residual.stride(1) != 1 or residual.dtype not in (torch.bfloat16, torch.float32)))):
+        raise ValueError(f"the residual rows are [{T}, {n_out}] in bfloat16 or float32")
+    if out is not None and (out.shape != (T, n_out) or out.stride(1) != 1 or (w.is_cuda and out.dtype != (torch.float32 if out_fp32 else torch.bfloat16))):
+        raise ValueError(f"the output is [{T}, {n_out}] in {'float32' if out_fp32 else 'bfloat16'}")
+    if not w.is_cuda:
+        xv = x.dequantize() if given else fp4_matrix.quantize(x, w.form).dequantize()
+        if pair:
+            y = ref.gate_up_act(xv, w.dequantize(), bias, "silu", True)
+        else:
+            y = ref.linear(xv, w.dequantize(), bias, residual, True)
+        y = y.to(torch.float32 if out_fp32 else torch.bfloat16 if given else x.dtype)
+        return y if out is None else out.copy_(y)
+    if out is None:
+        out = torch.empty(T, n_out, dtype=torch.float32 if out_fp32 else torch.bfloat16, device=w.device)
+    form = fp4_matrix.FORMS[w.form]
+    if given:
+        rows, ldx, x32, a = None, 0, 0, x.data
+    else:
+        if x.stride(1) != 1:
+            x = x.contiguous()
+        rows, ldx, x32 = x.data_ptr(), x.stride(0), int(x.dtype == torch.float32)
+        a = torch.empty(fp4_matrix.matrix_bytes(T, K, w.form), dtype=torch.uint8, device=w.device)
+    with _on(w.device):
+        _lib.check(_lib.lib().ogb_linear_fp4(rows, ldx, x32, a.data_ptr(), T, w.data.data_ptr(), N, K, form, out.data_ptr(), out.stride(0), int(out_fp32), int(pair),
+                                             _ptr(bias), _ptr(residual), residual.stride(0) if residual is not None else 0,
+                                             int(residual is not None and residual.dtype == torch.float32), workspace(w.device).status, _stream()), "linear_fp4")
+    return out
 
 
 def linear_act(x, w, act, out=None):
@@ -492,7 +582,21 @@ _PAIR_FLAGS = {"silu": 0, "relu": GEMM_PAIR_RELU, "gelu_tanh": GEMM_PAIR_GELU, "
 
 def gate_up_act(x, w, bias=None, act="silu", out=None, splits=0, interleaved=False, norm_eps=0.0):
     """act(x @ Wg.T) * (x @ Wu.T).  w is [2I, K]: stacked [Wg; Wu], or (interleaved=True) blocks of 64 gate
-    rows + 64 up rows as produced by interleave_gate_up (the layout the fused kernel needs).  norm_eps, splits: as in `linear`."""
+    rows + 64 up rows as produced by interleave_gate_up (the layout the fused kernel needs).  norm_eps, splits: as in `linear`.
+    w an Fp4Matrix: as in `linear`; its own `interleaved` tells the order of its rows."""
+    if isinstance(w, Fp4Matrix):
+        if norm_eps > 0:
+            if isinstance(x, Fp4Matrix):
+                raise ValueError("a norm cannot be folded into rows that are quantised already")
+            x = rms_scale(x, norm_eps)
+        if w.rows % 2:
+            raise ValueError(f"{w.rows} gate and up rows")
+        if act == "silu" and w.interleaved:
+            return _linear_fp4(x, w, bias, None, False, out, pair=True)
+        y = _linear_fp4(x, w, bias)
+        if w.interleaved:
+            y = y.view(-1, w.rows // 128, 2, 64).transpose(1, 2).reshape(-1, w.rows)
+        return act_mul(y.contiguous(), act, out)
     fused = None
     if norm_eps > 0:
         if not x.is_cuda:
@@ -860,6 +964,55 @@ def moe_combine(y: torch.Tensor, plan: MoePlan, residual=None) -> torch.Tensor:
     rc = _lib.lib().ogb_moe_combine(_ptr(y), y.stride(0), _ptr(plan.inv_pos), _ptr(plan.topk_w), plan.T, plan.k, y.shape[1], _ptr(residual),
                                     residual.stride(0) if residual is not None else 0, _ptr(out), out.stride(0), _stream())
     _lib.check(rc, "moe_combine")
+    return out
+
+
+MOE_FEW_TOKENS = 8                                                  # tokens that moe_few_tokens takes
+_FEW_RULES = {"selected": 0, "all": 1, "renormed": 2}
+_FEW_ACTS = {"silu": 1, "clamped": 2}
+
+
+def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, top: int, weights: str = "selected", act: str = "silu", alpha: float = 1.0,
+                   limit: float = 0.0):
+    """A whole mixture-of-experts layer for up to eight tokens: router product, choice of `top` experts per token (the largest logits, the lowest index among
+    equal ones), the chosen experts' gate / up products with the activation and down products, and the sum weighted by the routing weights.
+    x [T, H] bf16, 1 <= T <= 8; router_w [E, H] and router_b [E] (or None) bf16; gate_up_w [E, 2I, H] in interleave_experts_gate_up's order and
+    down_w [E, H, I]: bf16, or packed MXFP4 (Fp4Experts, both in the same form); gate_up_b [E, 2I] (in the same order) and down_b [E, H] bf16 or None.
+    weights "selected": softmax over the chosen logits; "all": over all; "renormed": over all, then over the chosen (the same numbers as "selected").
+    act "silu": silu(gate) * up; "clamped": g sigmoid(alpha g) (u + 1), where limit > 0 with gate <= limit and |up| <= limit.  Returns [T, H] bf16."""
+    if weights not in _FEW_RULES or act not in _FEW_ACTS:
+        raise ValueError(f"moe_few_tokens has no routing weights {weights!r} with the activation {act!r}")
+    if x.dim() != 2 or not 1 <= x.shape[0] <= MOE_FEW_TOKENS:
+        raise ValueError(f"moe_few_tokens takes 1 to {MOE_FEW_TOKENS} tokens, not {tuple(x.shape)}")
+    T, H = x.shape
+    E, two_i = gate_up_w.shape[0], gate_up_w.shape[1]
+    I = two_i // 2
+    if router_w.shape != (E, H) or tuple(gate_up_w.shape) != (E, 2 * I, H) or tuple(down_w.shape) != (E, H, I):
+        raise ValueError(f"router {tuple(router_w.shape)}, gate / up {tuple(gate_up_w.shape)} and down {tuple(down_w.shape)} do not fit {H} columns")
+    if I % 64 or H % 8 or not 1 <= top <= min(E, 32) or E > 1024:
+        raise ValueError(f"moe_few_tokens: {top} of {E} experts of width {I} on {H} columns: whole blocks of 64 features and 8 columns, at most 32 of 1024 experts")
+    for t, shape in ((router_b, (E,)), (gate_up_b, (E, 2 * I)), (down_b, (E, H))):
+        if t is not None and tuple(t.shape) != shape:
+            raise ValueError(f"a bias has the shape {tuple(t.shape)}: {shape} is wanted")
+    packed = isinstance(gate_up_w, Fp4Experts)
+    if packed != isinstance(down_w, Fp4Experts) or (packed and gate_up_w.half != down_w.half):
+        raise ValueError("moe_few_tokens wants both matrices of the experts in one form")
+    tensors = [t for t in (router_w, router_b, gate_up_b, down_b) if t is not None] + ([] if packed else [gate_up_w, down_w])
+    if any(t.device != x.device for t in tensors + [gate_up_w, down_w]):
+        raise ValueError("moe_few_tokens: tensors on different devices")
+    if not x.is_cuda:
+        return ref.moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, top, weights, act, alpha, limit)
+    if x.dtype != torch.bfloat16 or any(t.dtype != torch.bfloat16 or not t.is_contiguous() for t in tensors):
+        raise ValueError("moe_few_tokens takes contiguous bfloat16 weights and biases, and bfloat16 rows")
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    scratch = torch.empty(_lib.lib().ogb_moe_few_scratch_bytes(T, top, I), dtype=torch.uint8, device=x.device)
+    with _on(x.device):
+        _lib.check(_lib.lib().ogb_moe_few_tokens(x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),
+                                                 _ptr(gate_up_b), (down_w.packed if packed else down_w).data_ptr(), _ptr(down_b), out.data_ptr(), T, H, I, E, top,
+                                                 _FEW_RULES[weights], (1 if gate_up_w.half else 2) if packed else 0, _FEW_ACTS[act], float(alpha), float(limit),
+                                                 scratch.data_ptr(), _stream()), "moe_few_tokens")
     return out
 
 

@@ -435,6 +435,33 @@ def mamba2_scan(x, dt, neg_a, Bm, Cm, Dv, state, slots, cu_seqlens, past_lens):
 
 
 
+def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, top, weights, act, alpha, limit):
+    """A mixture-of-experts layer token by token (see ops.moe_few_tokens); gate / up rows in blocks of 64 + 64."""
+    logits = x.float() @ router_w.float().t()
+    if router_b is not None:
+        logits = logits + router_b.float()
+    vals, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
+    vals, ids = vals[:, :top], ids[:, :top]
+    share = torch.softmax(logits, dim=-1).gather(-1, ids) if weights == "all" else torch.softmax(vals, dim=-1)
+    expert = lambda w, e: (w[e] if torch.is_tensor(w) else w.dequantize(e)).float()
+    out = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+    for t in range(x.shape[0]):
+        for j, e in enumerate(ids[t].tolist()):
+            gu = expert(gate_up_w, e) @ x[t].float()
+            if gate_up_b is not None:
+                gu = gu + gate_up_b[e].float()
+            g, u = (v.reshape(-1) for v in gu.view(-1, 2, 64).unbind(1))
+            if act == "clamped":
+                if limit > 0:
+                    g, u = g.clamp(max=limit), u.clamp(min=-limit, max=limit)
+                h = g * torch.sigmoid(alpha * g) * (u + 1.0)
+            else:
+                h = torch.nn.functional.silu(g) * u
+            y = expert(down_w, e) @ h
+            out[t] += share[t, j] * (y if down_b is None else y + down_b[e].float())
+    return out.to(x.dtype)
+
+
 def head_project(x, w, heads, a_cols):
     """out[:, h * N + n] = sum_k x[:, h * a_cols + k] * w[h * N + n, k]."""
     N, K = w.shape[0] // heads, w.shape[1]

@@ -1,0 +1,180 @@
+"""4-bit floating-point rows and products against their definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from onnxruntime_genai_b200 import ops
+from onnxruntime_genai_b200.ops import fp4_matrix
+from test_fp4_matrix import rows_of
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def weight(N, K, form, seed=3, interleaved=False):
+    g = torch.Generator().manual_seed(seed)
+    w = fp4_matrix.quantize(torch.randn(N, K, generator=g) / math.sqrt(K), form)
+    c = w.codes()
+    return ops.Fp4Matrix.from_codes(c[:, 0::2] | c[:, 1::2] << 4, w.scales(), w.row_scales(), form, DEV, interleaved)
+
+
+def close(y, want, size, K):
+    """A product within its rounding to bf16 (half a step, 2^-8 of the value) and its fp32 sums: the tensor core adds the products of a block to the sum
+    in one go, which loses at most a last place (2^-23) of the sum of magnitudes `size`; K / 16 blocks, and a few steps for scales and additions."""
+    tol = (2.0 ** -8 if y.dtype == torch.bfloat16 else 0.0) * want.abs() + (K / 16 + 8) * 2.0 ** -23 * size + 1e-30
+    err = (y.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.3g} times what the roundings allow"
+
+
+# ------------------------------------------------------------------------------------------- rows
+@pytest.mark.parametrize("form", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["normal", "wide", "ties", "extremes"])
+@pytest.mark.parametrize("T,K", [(1, 32), (9, 96), (5, 2880), (130, 544), (3, 14336), (2, 20000 // 32 * 32)])
+def test_rows(T, K, kind, dtype, form):
+    x = rows_of(kind, T, K, dtype)
+    want, got = fp4_matrix.quantize(x, form), ops.quantize_fp4(x.to(DEV), form)
+    finite = torch.isfinite(x.float()).all(-1)
+    # values, not bytes: a zero may carry either sign, and a block of zeros any scale
+    nan_rows = lambda m: torch.nan_to_num(m.dequantize().cpu(), nan=7e30)
+    assert torch.equal(nan_rows(got), nan_rows(want))
+    assert torch.equal(torch.isnan(got.row_scales().cpu()), ~finite)
+    assert torch.equal(got.dequantize(torch.bfloat16).cpu().nan_to_num(7.0), want.dequantize(torch.bfloat16).nan_to_num(7.0))
+
+
+def test_rows_with_strides():
+    x = rows_of("normal", 40, 704, torch.bfloat16).to(DEV)
+    for v in (x[:, 64:320], x[::3, 1:257], x[:, :512].t()[:, :32]):
+        assert torch.equal(ops.quantize_fp4(v).dequantize(), ops.quantize_fp4(v.contiguous().clone()).dequantize())
+    assert ops.quantize_fp4(x[:0, :64]).dequantize().shape == (0, 64)
+
+
+def test_padding_of_the_last_k_block_is_zero():
+    m = ops.quantize_fp4(rows_of("normal", 3, 272, torch.bfloat16).to(DEV))
+    c, s = fp4_matrix.Fp4Matrix(m.data, 3, 512, "nvfp4"), None
+    assert not c.codes()[:, 272:].any() and not c.scales()[:, 17:].any()
+
+
+# ------------------------------------------------------------------------------------------- products
+SHAPES = [(1, 128, 64), (1, 6144, 4096), (2, 65, 96), (7, 4096, 14336), (16, 28672, 512), (17, 1000, 2880), (31, 200, 320), (33, 129, 256), (64, 4096, 1024), (65, 777, 288),
+          (128, 512, 2048), (129, 640, 544), (200, 300, 1024), (256, 256, 256), (300, 5120, 2880), (513, 1111, 320), (777, 2880, 640), (1025, 4096, 512)]
+
+
+@pytest.mark.parametrize("form", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("T,N,K", SHAPES)
+def test_products(T, N, K, form):
+    x = rows_of("wide" if T % 2 else "normal", T, K, torch.bfloat16).to(DEV)
+    w = weight(N, K, form)
+    xq, wq = ops.quantize_fp4(x, form).dequantize().double(), w.dequantize().double()
+    want, size = xq @ wq.T, xq.abs() @ wq.abs().T
+    close(ops.linear(x, w), want, size, K)
+    close(ops.linear(x, w, out_fp32=True), want, size, K)
+    g = torch.Generator().manual_seed(T)
+    bias, res = torch.randn(N, generator=g).to(torch.bfloat16).to(DEV), torch.randn(T, N + 3, generator=g).to(DEV)[:, :N]
+    want, size = want + bias.double() + res.double(), size + bias.double().abs() + res.double().abs()
+    close(ops.linear(x, w, bias, res, out_fp32=True), want, size, K)
+    rb = res.to(torch.bfloat16)
+    close(ops.linear(x, w, bias, rb), want - res.double() + rb.double(), size, K)
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("form", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("T,N,K", [(1, 128, 64), (3, 1152, 2880), (16, 28672, 320), (40, 512, 1024), (150, 5760, 288), (300, 384, 512), (600, 1280, 2048)])
+def test_gated_products(T, N, K, form):
+    x = rows_of("normal", T, K, torch.bfloat16).to(DEV)
+    w = weight(N, K, form, interleaved=True)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16).to(DEV)
+    xq, wq = ops.quantize_fp4(x, form).dequantize().double(), w.dequantize().double()
+    y, size = xq @ wq.T + bias.double(), xq.abs() @ wq.abs().T + bias.double().abs()
+    split = lambda t: (v.reshape(T, N // 2) for v in t.view(T, N // 128, 2, 64).unbind(2))
+    (g, u), (sg, su) = split(y), split(size)
+    got = ops.gate_up_act(x, w, bias).double()
+    want = torch.nn.functional.silu(g) * u
+    # silu's slope is at most 1.1; its own fp32 steps (an exponential and a division of a few last places each): 2^-20 of the result
+    d = (K / 16 + 8) * 2.0 ** -23
+    tol = 2.0 ** -8 * want.abs() + d * (1.1 * sg * (u.abs() + d * su) + g.abs() * su) + 2.0 ** -20 * want.abs() + 1e-30
+    assert bool(((got - want).abs() <= tol).all())
+    relu = ops.gate_up_act(x, w, bias, act="relu").double()
+    rw = torch.relu(g) * u
+    assert bool(((relu - rw).abs() <= 3 * 2.0 ** -8 * rw.abs() + 2 * d * (sg * (u.abs() + d * su) + g.abs() * su) + 1e-30).all())
+    ops.check_kernel_status()
+
+
+def test_quantised_rows_serve_several_products():
+    x = rows_of("normal", 70, 576, torch.bfloat16).to(DEV)
+    q = ops.quantize_fp4(x)
+    for N in (64, 300):
+        w = weight(N, 576, "nvfp4")
+        assert torch.equal(ops.linear(q, w), ops.linear(x, w))
+
+
+def test_rows_that_are_not_numbers_stay_to_themselves():
+    for T in (5, 200):
+        x = rows_of("normal", T, 512, torch.bfloat16).to(DEV)
+        w = weight(256, 512, "nvfp4")
+        ref = ops.linear(x, w)
+        y = x.clone()
+        y[1, 7], y[T - 2, 400] = math.inf, math.nan
+        got = ops.linear(y, w)
+        keep = torch.ones(T, dtype=torch.bool, device=DEV)
+        keep[1] = keep[T - 2] = False
+        assert torch.equal(got[keep], ref[keep]) and bool(torch.isnan(got[~keep]).all())
+
+
+def test_output_ranges_are_left_as_they_were():
+    for T, N in ((3, 100), (140, 100)):
+        x, w = rows_of("normal", T, 256, torch.bfloat16).to(DEV), weight(N, 256, "nvfp4")
+        big = torch.full((T + 2, N + 7), 3.0, dtype=torch.bfloat16, device=DEV)
+        ops.linear(x, w, out=big[1:T + 1, 3:N + 3])
+        assert torch.equal(big[1:T + 1, 3:N + 3], ops.linear(x, w))
+        big[1:T + 1, 3:N + 3] = 3.0
+        assert bool((big == 3.0).all())
+
+
+def test_unaligned_rows_and_fp32_rows():
+    for T in (4, 180):
+        wide = rows_of("normal", T, 300, torch.bfloat16).to(DEV)
+        w = weight(192, 256, "nvfp4")
+        assert torch.equal(ops.linear(wide[:, 3:259], w), ops.linear(wide[:, 3:259].contiguous(), w))
+        assert torch.equal(ops.linear(wide[:, :256].float(), w), ops.linear(wide[:, :256], w))
+
+
+def test_same_results_every_time_and_from_graphs():
+    for T, N, K in ((1, 512, 4096), (20, 640, 8192), (300, 1024, 1024)):
+        x, w = rows_of("normal", T, K, torch.bfloat16).to(DEV), weight(N, K, "nvfp4")
+        first = ops.linear(x, w)
+        for _ in range(5):
+            assert torch.equal(ops.linear(x, w), first)
+        side = torch.cuda.Stream()
+        graphs = []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            side.wait_stream(torch.cuda.current_stream())
+            with ops.graph_capture(g, stream=side):
+                y = ops.linear(x, w)
+            graphs.append((g, y))
+        torch.cuda.synchronize()
+        x2 = rows_of("normal", T, K, torch.bfloat16, seed=9).to(DEV)
+        want = ops.linear(x2, w)
+        x.copy_(x2)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for s, (g, _) in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want) for _, y in graphs)
+
+
+def test_refusals_of_device_tensors():
+    w = weight(64, 64, "nvfp4")
+    x = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="different devices"):
+        ops.linear(x.cpu(), w)
+    with pytest.raises(ValueError, match="bias"):
+        ops.linear(x, w, bias=torch.zeros(64, device=DEV))
+    with pytest.raises(ValueError, match="output"):
+        ops.linear(x, w, out=torch.zeros(2, 64, device=DEV))
+    with pytest.raises(ValueError, match="residual"):
+        ops.linear(x, w, residual=torch.zeros(2, 64, dtype=torch.float16, device=DEV))

@@ -1,0 +1,149 @@
+"""The expert layer for few tokens against its definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from onnxruntime_genai_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def layer(T, E, H, I, kind, bias, seed=0):
+    """Arguments of the call, and the experts' numbers in 64 bits with the gate and up rows of every expert stacked."""
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16).to(DEV)
+    order = lambda t: ops.interleave_experts_gate_up(t, fused_interleaved=False)
+    p = dict(x=n(T, H), router_w=n(E, H) / math.sqrt(H), router_b=n(E) if bias else None)
+    gu_b, d_b = (n(E, 2 * I), n(E, H)) if bias else (None, None)
+    if kind == "bf16":
+        gu, d = n(E, 2 * I, H) / math.sqrt(H), n(E, H, I) / math.sqrt(I)
+        p.update(gate_up_w=order(gu), down_w=d)
+    else:
+        def packed(N, K, rows):
+            codes = torch.randint(0, 16, (E, N, K), dtype=torch.uint8, generator=g)
+            sc = torch.randint(117, 122, (E, N, K // 32), dtype=torch.uint8, generator=g)
+            if kind == "fp4 bf16 form":
+                sc[0, 0, 0] = 90          # below the fp16 form's range
+            half = kind != "fp4 bf16 form"
+            v = ops.Fp4Experts.from_codes(codes, sc, "cpu", half=half).dequantize().to(DEV)
+            return ops.Fp4Experts.from_codes(rows(codes), rows(sc), DEV, half=half), v
+        (p["gate_up_w"], gu), (p["down_w"], d) = packed(2 * I, H, order), packed(H, I, lambda t: t)
+    p.update(gate_up_b=order(gu_b) if bias else None, down_b=d_b)
+    return p, dict(gate_up=gu, gate_up_b=gu_b, down=d, down_b=d_b)
+
+
+def exact(p, w, top, weights, act, alpha, limit):
+    """The layer in 64 bits, and how far the call may be off: relative steps of 2^-8 for what it rounds to 16 bits (the activations between the products, the
+    result; packed experts in fp16 form: 2^-11, covered by that), fp32 sums of n products 2^-24 n of the sum of magnitudes."""
+    x = p["x"].double()
+    T, H = x.shape
+    I = w["down"].shape[2]
+    logits = x @ p["router_w"].double().T + (p["router_b"].double() if p["router_b"] is not None else 0)
+    out, tol = torch.zeros_like(x), torch.zeros_like(x)
+    for t in range(T):
+        vals, ids = torch.sort(logits[t], descending=True, stable=True)
+        share = torch.softmax(logits[t], -1)[ids[:top]] if weights == "all" else torch.softmax(vals[:top], -1)
+        for s, e in zip(share, ids[:top].tolist()):
+            m = w["gate_up"][e].double()
+            gu, size = m @ x[t], m.abs() @ x[t].abs()
+            if w["gate_up_b"] is not None:
+                gu, size = gu + w["gate_up_b"][e].double(), size + w["gate_up_b"][e].double().abs()
+            g, u, dg, du = gu[:I], gu[I:], H * 2.0 ** -24 * size[:I], H * 2.0 ** -24 * size[I:]
+            if act == "clamped":
+                if limit > 0:
+                    g, u = g.clamp(max=limit), u.clamp(-limit, limit)
+                sg = torch.sigmoid(alpha * g)
+                h, dh = g * sg * (u + 1), (1 + alpha * g.abs()) * dg * (u + 1).abs() + g.abs() * du
+            else:
+                sg = torch.sigmoid(g)
+                h, dh = g * sg * u, 1.1 * dg * u.abs() + g.abs() * du
+            dh = dh + 2.0 ** -8 * h.abs() + 2.0 ** -20 * h.abs()
+            d = w["down"][e].double()
+            y, dy = d @ h, d.abs() @ dh + I * 2.0 ** -24 * (d.abs() @ h.abs())
+            if w["down_b"] is not None:
+                y = y + w["down_b"][e].double()
+            out[t] += s * y
+            tol[t] += s * dy + 2.0 ** -18 * s * y.abs()          # routing weight: logits in fp32, an exponential
+    return out, tol + 2.0 ** -8 * out.abs() + 1e-6
+
+
+KINDS = ["bf16", "fp4", "fp4 bf16 form"]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T,E,top,H,I,weights,act", [
+    (1, 8, 2, 64, 64, "selected", "silu"), (1, 32, 4, 2880, 2880, "selected", "clamped"), (2, 128, 8, 2048, 768, "renormed", "silu"),
+    (8, 8, 2, 512, 1024, "selected", "silu"), (5, 60, 4, 320, 192, "all", "silu"), (8, 4, 4, 128, 448, "renormed", "clamped"),
+    (7, 32, 4, 704, 576, "selected", "clamped"), (3, 1, 1, 192, 64, "all", "silu"), (8, 300, 32, 64, 64, "selected", "silu")])
+def test_layer(T, E, top, H, I, weights, act, kind):
+    p, w = layer(T, E, H, I, kind, act == "clamped")
+    args = dict(top=top, weights=weights, act=act, alpha=1.702 if act == "clamped" else 1.0, limit=1.5 if act == "clamped" else 0.0)
+    got = ops.moe_few_tokens(**p, **args)
+    want, tol = exact(p, w, **args)
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), f"off by {float((err / tol).max()):.3g} times what the roundings allow"
+    for t in range(T):                  # a token's result does not go by its neighbours
+        alone = ops.moe_few_tokens(**{**p, "x": p["x"][t:t + 1]}, **args)
+        assert bool(((alone.double() - want[t:t + 1]).abs() <= tol[t:t + 1]).all())
+    assert torch.equal(ops.moe_few_tokens(**p, **args), got)
+
+
+def test_columns_that_are_no_whole_vectors():
+    p, w = layer(4, 8, 72, 128, "bf16", False)
+    args = dict(top=2, weights="selected", act="silu", alpha=1.0, limit=0.0)
+    want, tol = exact(p, w, **args)
+    wide = torch.zeros(4, 99, dtype=torch.bfloat16, device=DEV)
+    wide[:, 3:75] = p["x"]
+    for x in (p["x"], wide[:, 3:75], p["x"].t().contiguous().t()):
+        assert bool(((ops.moe_few_tokens(**{**p, "x": x}, **args).double() - want).abs() <= tol).all())
+
+
+def test_all_tokens_at_one_expert_and_equal_logits():
+    p, w = layer(8, 16, 256, 128, "bf16", False)
+    p["router_w"] = torch.zeros_like(p["router_w"])
+    args = dict(top=3, weights="selected", act="silu", alpha=1.0, limit=0.0)
+    want, tol = exact(p, w, **args)
+    p["gate_up_w"][3:] = math.nan                     # experts beyond the first three are not looked at
+    p["down_w"][3:] = math.nan
+    assert bool(((ops.moe_few_tokens(**p, **args).double() - want).abs() <= tol).all())
+
+
+def test_rows_that_are_not_numbers_stay_to_themselves():
+    p, _ = layer(6, 8, 128, 64, "bf16", True)
+    args = dict(top=2, weights="renormed", act="silu")
+    ref = ops.moe_few_tokens(**p, **args)
+    p["x"] = p["x"].clone()
+    p["x"][2, 5], p["x"][4, 0] = math.nan, math.inf
+    got = ops.moe_few_tokens(**p, **args)
+    keep = [0, 1, 3, 5]
+    assert torch.equal(got[keep], ref[keep]) and bool(torch.isnan(got[2]).all())
+
+
+def test_two_graphs_at_once():
+    p, _ = layer(4, 32, 512, 256, "fp4", True)
+    args = dict(top=4, act="clamped", alpha=1.702, limit=7.0)
+    first = ops.moe_few_tokens(**p, **args)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with ops.graph_capture(g):
+            y = ops.moe_few_tokens(**p, **args)
+        graphs.append((g, y, torch.cuda.Stream()))
+    for _ in range(3):
+        for g, _, s in graphs:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, first) for _, y, _ in graphs)
+
+
+def test_refusals_of_device_tensors():
+    p, _ = layer(2, 8, 64, 64, "bf16", True)
+    for kw in (dict(x=p["x"].float()), dict(router_w=p["router_w"].float()), dict(down_b=p["down_b"].float()), dict(gate_up_w=p["gate_up_w"].transpose(0, 1).contiguous().transpose(0, 1))):
+        with pytest.raises(ValueError, match="bfloat16"):
+            ops.moe_few_tokens(**{**p, **kw}, top=2)
+    with pytest.raises(ValueError, match="different devices"):
+        ops.moe_few_tokens(**{**p, "router_b": p["router_b"].cpu()}, top=2)
