@@ -346,7 +346,8 @@ int ogb_quantize_fp4(const void* x, long long ldx, int x_fp32, int rows, int K, 
 int ogb_dequantize_fp4(const void* data, int rows, int K, int form, void* out, long long ldo, int out_fp32, void* stream);
 // x != null: these rows are quantised into a_data first; null: a_data holds quantised rows.  pair: silu(gate) * up of blocks of 64 + 64 weight rows
 int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T, const void* w_data, int N, int K, int form, void* out, long long ldc,
-                   int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, void* stream);
+                   int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, int sm_count,
+                   void* stream);
 
 // ---- moe_few.cu (a whole expert layer for up to eight tokens; rule: mode of ogb_moe_topk; weights 0: bf16, 1 / 2: packed MXFP4 in its fp16 / bf16 form;
 // act 1: silu(gate) * up, 2: clamped SwiGLU; gate_up in blocks of 64 gate + 64 up rows)

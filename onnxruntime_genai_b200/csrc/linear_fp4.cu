@@ -1,13 +1,21 @@
 // Linear layers on 4-bit floating-point rows and weights (layout: fp4_matrix.cuh):
 //   C[t, n] = a_row[t] * w_row[n] * sum_blocks a_scale * w_scale * sum_k a_code * w_code   (+ bias, residual, or the gated activation)
+//
+// Both operands go to the block-scaled tensor-core product (`tcgen05.mma.kind::mxf4nvf4.block_scale`) as they are: codes from shared memory, block
+// scales from tensor memory, fp32 accumulators.  Weights are the M operand (128 rows a CTA), tokens the N operand.
+//
+// Few tokens (linear_fp4_kernel): bound by the weights' bytes.  A CTA holds one tile of 128 weight rows x BT tokens of a part of the k-blocks; the parts of a
+// tile form a cluster that sums its accumulators through distributed shared memory, always in the same order.
+#include "gemm_common.cuh"
 #include "fp4_matrix.cuh"
 #include "kernels.h"
+#include "packed_weights.cuh"
 
 namespace ogb {
 
 struct Fp4LinearArgs {
   Fp4View a, w;
-  int N;
+  int N, n_out;
   void* C;
   long long ldc;
   int out_fp32, pair;
@@ -15,46 +23,303 @@ struct Fp4LinearArgs {
   const void* residual;
   long long ldr;
   int res_fp32;
+  int whole;                    // every eight columns of an output and residual row are aligned for 16-byte accesses
+  int splits, kb_per_split;
+  int early;                    // weights may be fetched before the kernel in front has finished (it does not write them, nor do those before it)
+  int* status;
+  int pdl;
 };
 
-constexpr int TILE = 16;
+constexpr int FP4_TILE = 128;                                    // weight rows of a CTA
+constexpr int FP4_W_BYTES = FP4_TILE * 128;                      // codes of a k-block
+__host__ __device__ constexpr int fp4_sf_bytes(int form) { return fp4_steps(form) * FP4_SCALE_STEP; }
+
+// ------------------------------------------------------------------------------- tensor-core wrappers
+// Instruction descriptor of the block-scaled e2m1 products: both operands e2m1 and K-major; bit 23 tells e8m0 from e4m3 scales; the scale ids say which of
+// a column's four bytes belong to this instruction (0, or 2 where it takes two).
+__host__ __device__ constexpr uint32_t fp4_idesc(int form, int m, int n, int id) {
+  return (1u << 7) | (1u << 10) | (uint32_t(id) << 4) | (uint32_t(n >> 3) << 17) | (form == FP4_MX ? 1u << 23 : 0u) | (uint32_t(m >> 7) << 27) | (uint32_t(id) << 29);
+}
+// Shared-memory descriptor of 32 x 16 bytes without swizzle (groups of eight rows 128 bytes apart): what a copy of scales reads.
+__device__ __forceinline__ uint64_t fp4_scale_desc(uint32_t addr) {
+  return uint64_t((addr & 0x3FFFF) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+template <int CTAS>
+__device__ __forceinline__ void fp4_copy_scales(uint32_t taddr, uint64_t desc) {     // 512 bytes -> four columns, in all four lane quarters
+  if constexpr (CTAS == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+#define FP4_MMA(GROUP, VEC)                                                                                                              \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                                           \
+               "tcgen05.mma.cta_group::" GROUP ".kind::mxf4nvf4.block_scale.scale_vec::" VEC " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"           \
+               ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate) : "memory")
+template <int CTAS, int FORM>
+__device__ __forceinline__ void fp4_mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  if constexpr (CTAS == 1) { if constexpr (FORM == FP4_NV) FP4_MMA("1", "4X"); else FP4_MMA("1", "2X"); }
+  else { if constexpr (FORM == FP4_NV) FP4_MMA("2", "4X"); else FP4_MMA("2", "2X"); }
+}
+
+// ------------------------------------------------------------------------------- results
+// Eight columns of token row m: residual and store.
+__device__ __forceinline__ void fp4_store8(const Fp4LinearArgs& p, int m, int col, float (&v)[8]) {
+  const int n = min(8, p.n_out - col);
+  const bool whole = p.whole && n == 8;
+  if (p.residual) {
+    if (p.res_fp32) {
+      const float* r = static_cast<const float*>(p.residual) + m * p.ldr + col;
+      if (whole) {
+        const float4 x = reinterpret_cast<const float4*>(r)[0], y = reinterpret_cast<const float4*>(r)[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < n) v[j] += r[j];
+      }
+    } else {
+      const __nv_bfloat16* r = static_cast<const __nv_bfloat16*>(p.residual) + m * p.ldr + col;
+      if (whole) {
+        const uint4 q = *reinterpret_cast<const uint4*>(r);
+        const float2 x0 = unpack_bf16x2(q.x), x1 = unpack_bf16x2(q.y), x2 = unpack_bf16x2(q.z), x3 = unpack_bf16x2(q.w);
+        v[0] += x0.x; v[1] += x0.y; v[2] += x1.x; v[3] += x1.y; v[4] += x2.x; v[5] += x2.y; v[6] += x3.x; v[7] += x3.y;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < n) v[j] += bf2f(r[j]);
+      }
+    }
+  }
+  if (p.out_fp32) {
+    float* c = static_cast<float*>(p.C) + m * p.ldc + col;
+    if (whole) {
+      reinterpret_cast<float4*>(c)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(c)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (j < n) c[j] = v[j];
+    }
+  } else {
+    __nv_bfloat16* c = static_cast<__nv_bfloat16*>(p.C) + m * p.ldc + col;
+    if (whole) {
+      *reinterpret_cast<uint4*>(c) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) if (j < n) c[j] = f2bf(v[j]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- few tokens
+template <int BT, int FORM>
+struct Fp4Cfg {
+  static constexpr int SF = fp4_sf_bytes(FORM);
+  static constexpr int X_OFF = FP4_W_BYTES, SFW_OFF = X_OFF + BT * 128, SFX_OFF = SFW_OFF + SF;
+  static constexpr int STAGE = SFX_OFF + SF;                                     // codes of weights and tokens, scales of weights and of 128 tokens
+  static constexpr int STAGES = 110 * 1024 / STAGE < 8 ? 110 * 1024 / STAGE : 8;  // two CTAs per SM
+  static constexpr int SF_COL = BT < 32 ? 32 : BT;                                // first tensor-memory column of the scales: two sets of 16 + 16
+  static constexpr int COLS = SF_COL + 64 <= 128 ? 128 : 256;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
+  static_assert(STAGE % 1024 == 0 && BT * FP4_TILE * 4 <= STAGES * STAGE && 2 * (SMEM + 1024) <= 228 * 1024, "shared memory");
+};
+
+template <int BT, int FORM>
+__global__ void __launch_bounds__(192, 2) linear_fp4_kernel(const Fp4LinearArgs p) {
+  using Cfg = Fp4Cfg<BT, FORM>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE);
+  uint64_t* empty = full + Cfg::STAGES;
+  uint64_t* accum = empty + Cfg::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int n_tile = blockIdx.x, row0 = blockIdx.y * BT, rows = min(BT, p.a.rows - row0);
+  const int kb0 = blockIdx.z * p.kb_per_split, num = max(0, min(p.kb_per_split, p.w.num_kb - kb0));
+  auto fail = [&](int code) { atomicMax(p.status, code); *abort_flag = 1; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    mbar_init(accum, 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) { tmem_alloc(tmem_slot, Cfg::COLS); tmem_relinquish(); }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (p.pdl) pdl_launch_dependents();
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- copies
+    const uint8_t* w = p.w.codes + (long long)n_tile * FP4_W_BYTES;
+    const uint8_t* sw = p.w.scales + (long long)n_tile * Cfg::SF;
+    const uint8_t* x = p.a.codes + (long long)row0 * 128;
+    const uint8_t* sx = p.a.scales + (long long)(row0 >> 7) * Cfg::SF;
+    const long long w_step = (long long)p.w.padded * 128, x_step = (long long)p.a.padded * 128;
+    const long long sw_step = (long long)(p.w.padded >> 7) * Cfg::SF, sx_step = (long long)(p.a.padded >> 7) * Cfg::SF;
+    auto weights = [&](int i, int s) {
+      uint8_t* st = smem + s * Cfg::STAGE;
+      mbar_expect_tx(&full[s], Cfg::STAGE);
+      bulk_copy_g2s(st, w + (kb0 + i) * w_step, FP4_W_BYTES, &full[s]);
+      bulk_copy_g2s(st + Cfg::SFW_OFF, sw + (kb0 + i) * sw_step, Cfg::SF, &full[s]);
+    };
+    auto tokens = [&](int i, int s) {
+      uint8_t* st = smem + s * Cfg::STAGE;
+      bulk_copy_g2s(st + Cfg::X_OFF, x + (kb0 + i) * x_step, BT * 128, &full[s]);
+      bulk_copy_g2s(st + Cfg::SFX_OFF, sx + (kb0 + i) * sx_step, Cfg::SF, &full[s]);
+    };
+    const int ahead = min(num, Cfg::STAGES);
+    if (p.pdl && !p.early) pdl_wait();
+    if (elect_one()) for (int i = 0; i < ahead; ++i) weights(i, i);
+    __syncwarp();
+    if (p.pdl && p.early) pdl_wait();
+    if (elect_one()) for (int i = 0; i < ahead; ++i) tokens(i, i);
+    __syncwarp();
+    bool ok = true;
+    int s = 0, filled = ahead;
+    uint32_t ph = 0;
+    for (int i = ahead; i < num; ++i) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ph, abort_flag));
+      if (!ok) { fail(OGB_ERR_WAIT_TMA); break; }
+      if (elect_one()) { weights(i, s); tokens(i, s); }
+      __syncwarp();
+      ++filled;
+      if (++s == Cfg::STAGES) { s = 0; ph ^= 1; }
+    }
+    if (!ok || *abort_flag) {     // copies in flight still write this shared memory: give them time to land
+      volatile int never = 0;
+      for (int i = max(0, filled - Cfg::STAGES); i < filled; ++i) mbar_wait_bounded(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, &never, 200000000ull);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < num; ++i) {
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag))) { fail(OGB_ERR_WAIT_TMA); break; }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t base = smem_u32(smem + s * Cfg::STAGE), sf = tmem + Cfg::SF_COL + (i & 1) * 32;
+        const uint64_t dw = umma_desc_sw128(base), dx = umma_desc_sw128(base + Cfg::X_OFF);
+        const uint64_t dsw = fp4_scale_desc(base + Cfg::SFW_OFF), dsx = fp4_scale_desc(base + Cfg::SFX_OFF);
+#pragma unroll
+        for (int j = 0; j < fp4_steps(FORM); ++j) {
+          fp4_copy_scales<1>(sf + j * 4, dsw + j * (FP4_SCALE_STEP >> 4));
+          fp4_copy_scales<1>(sf + 16 + j * 4, dsx + j * (FP4_SCALE_STEP >> 4));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {                       // 64 k values: 32 bytes of a row
+          const int col = FORM == FP4_NV ? j * 4 : (j >> 1) * 4;
+          fp4_mma<1, FORM>(tmem, dw + j * 2, dx + j * 2, fp4_idesc(FORM, FP4_TILE, BT, FORM == FP4_NV ? 0 : (j & 1) * 2), sf + col, sf + 16 + col,
+                           i > 0 || j > 0 ? 1u : 0u);
+        }
+        umma_commit(&empty[s]);
+        if (i == num - 1) umma_commit(accum);
+      }
+      __syncwarp();
+      if (++s == Cfg::STAGES) { s = 0; ph ^= 1; }
+    }
+  }
+  // ------------------------------------------------------------------ accumulators to shared memory, sums over the cluster, results (warps 2..5)
+  float* part = reinterpret_cast<float*>(smem);               // [BT][128] in the stages: all copies and products are done when the accumulator is
+  const int et = int(threadIdx.x) - 64;
+  if (warp >= 2) {
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    if (num > 0) {
+      if (!mbar_wait_bounded(accum, 0, abort_flag, 4000000000ull)) fail(OGB_ERR_WAIT_MMA);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (*abort_flag == 0) {
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < BT && c0 < rows; c0 += 16) {
+          uint32_t r[16];
+          tmem_ld16(tmem + (uint32_t(quarter * 32) << 16) + c0, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c0 + j) * FP4_TILE + row] = __uint_as_float(r[j]);
+        }
+      }
+    }
+    if (p.pdl) pdl_wait();
+  }
+  __syncwarp();
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync_all(); else __syncthreads();
+  if (warp >= 2 && *abort_flag == 0) {
+    const int rank = p.splits > 1 ? int(cluster_ctarank()) : 0;
+    const int per = (rows + p.splits - 1) / p.splits, first = min(rows, rank * per), last = min(rows, first + per);   // tokens that this CTA finishes
+    const int segs = p.pair ? 8 : 16, used = min(p.splits, (p.w.num_kb + p.kb_per_split - 1) / p.kb_per_split);
+    const uint32_t at = smem_u32(part);
+    auto sum8 = [&](int m, int n, float scale, float (&v)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      for (int q = 0; q < used; ++q) {
+        const uint32_t a = p.splits > 1 ? dsmem_addr(at + uint32_t(m * FP4_TILE + n) * 4, uint32_t(q)) : 0u;
+        const float4* l = reinterpret_cast<const float4*>(part + m * FP4_TILE + n);
+        const float4 x = p.splits > 1 ? ld_dsmem_f32x4(a) : l[0], y = p.splits > 1 ? ld_dsmem_f32x4(a + 16) : l[1];
+        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+      }
+      const int g = n_tile * FP4_TILE + n;                     // (row scales are padded to whole tiles)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] *= scale * p.w.row_scale[g + j];
+        if (p.bias && g + j < p.N) v[j] += bf2f(p.bias[g + j]);
+      }
+    };
+    for (int i = et; i < (last - first) * segs; i += 128) {
+      const int m = first + i / segs, seg = i % segs * 8, col = n_tile * (p.pair ? 64 : 128) + seg;
+      if (col >= p.n_out) continue;
+      const float scale = p.a.row_scale[row0 + m];
+      float v[8];
+      sum8(m, seg, scale, v);
+      if (p.pair) {
+        float u[8];
+        sum8(m, seg + 64, scale, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = silu(v[j]) * u[j];
+      }
+      fp4_store8(p, row0 + m, col, v);
+    }
+  }
+  __syncwarp();
+  if (p.splits > 1) cluster_sync_all(); else __syncthreads();   // no CTA leaves while another reads its sums
+  if (warp == 1) tmem_dealloc(tmem, Cfg::COLS);
+}
+
+template <int BT, int FORM>
+static int LaunchFew(Fp4LinearArgs p, int splits, cudaStream_t stream) {
+  using Cfg = Fp4Cfg<BT, FORM>;
+  static bool configured[OGB_MAX_DEVICES] = {};
+  if (!set_max_dyn_smem(linear_fp4_kernel<BT, FORM>, Cfg::SMEM, configured)) return -3;
+  p.splits = splits;
+  p.kb_per_split = (p.w.num_kb + splits - 1) / splits;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(p.w.padded / FP4_TILE), unsigned((p.a.rows + BT - 1) / BT), unsigned(splits));
+  cfg.blockDim = dim3(192);
+  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (splits > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim = {1, 1, unsigned(splits)};
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, linear_fp4_kernel<BT, FORM>, p) == cudaSuccess ? 0 : -4;
+}
+
 template <int FORM>
-__global__ void linear_fp4_simple_kernel(Fp4LinearArgs p) {
-  constexpr int B = FORM == FP4_NV ? 16 : 32;
-  __shared__ float sa[TILE][FP4_KB], sw[2][TILE][FP4_KB];
-  const int tx = threadIdx.x % TILE, ty = threadIdx.x / TILE;
-  const int n_out = p.pair ? p.N / 2 : p.N, t0 = blockIdx.y * TILE, col = blockIdx.x * TILE + tx;
-  float acc[2] = {0.f, 0.f};
-  auto value = [&](const Fp4View& m, int kb, int r, int k) {
-    if (r >= m.rows) return 0.f;
-    const uint32_t byte = m.codes[fp4_code_at(m, kb, r, k >> 5) + ((k & 31) >> 1)];
-    return fp4_value((k & 1) ? byte >> 4 : byte & 15u) * fp4_scale(FORM, m.scales[fp4_scale_at(m, FORM, kb, r, (k / B) >> 2, (k / B) & 3)]);
-  };
-  auto weight_row = [&](int c) { return p.pair ? c / 64 * 128 + c % 64 : c; };   // gate row of an output column; its up row is 64 further
-  for (int kb = 0; kb < p.a.num_kb; ++kb) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < TILE * FP4_KB; i += blockDim.x) {
-      const int r = i / FP4_KB, k = i % FP4_KB, wr = weight_row(blockIdx.x * TILE + r);
-      sa[r][k] = value(p.a, kb, t0 + r, k);
-      sw[0][r][k] = value(p.w, kb, wr, k);
-      if (p.pair) sw[1][r][k] = value(p.w, kb, wr + 64, k);
-    }
-    __syncthreads();
-    for (int k = 0; k < FP4_KB; ++k) {
-      acc[0] += sa[ty][k] * sw[0][tx][k];
-      if (p.pair) acc[1] += sa[ty][k] * sw[1][tx][k];
-    }
-  }
-  const int t = t0 + ty, wr = weight_row(col);
-  if (t >= p.a.rows || col >= n_out) return;
-  const float s = p.a.row_scale[t];
-  float v = acc[0] * s * p.w.row_scale[wr] + (p.bias ? bf2f(p.bias[wr]) : 0.f);
-  if (p.pair) {
-    const float u = acc[1] * s * p.w.row_scale[wr + 64] + (p.bias ? bf2f(p.bias[wr + 64]) : 0.f);
-    v = v / (1.f + __expf(-v)) * u;
-  }
-  if (p.residual) v += p.res_fp32 ? static_cast<const float*>(p.residual)[t * p.ldr + col] : bf2f(static_cast<const __nv_bfloat16*>(p.residual)[t * p.ldr + col]);
-  if (p.out_fp32) static_cast<float*>(p.C)[t * p.ldc + col] = v; else static_cast<__nv_bfloat16*>(p.C)[t * p.ldc + col] = f2bf(v);
+static int LaunchLinear(const Fp4LinearArgs& p, int sm_count, cudaStream_t stream) {
+  const int T = p.a.rows, bt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  const int tiles = p.w.padded / FP4_TILE * ((T + bt - 1) / bt);
+  const int splits = max(1, min(min(8, p.w.num_kb), 2 * sm_count / tiles));
+  if (bt == 16) return LaunchFew<16, FORM>(p, splits, stream);
+  if (bt == 32) return LaunchFew<32, FORM>(p, splits, stream);
+  if (bt == 64) return LaunchFew<64, FORM>(p, splits, stream);
+  return LaunchFew<128, FORM>(p, splits, stream);
 }
 
 }  // namespace ogb
@@ -62,19 +327,35 @@ __global__ void linear_fp4_simple_kernel(Fp4LinearArgs p) {
 using namespace ogb;
 
 OGB_API int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T, const void* w_data, int N, int K, int form, void* out, long long ldc,
-                           int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, void* stream) {
+                           int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, int sm_count, void* stream) {
   if (!w_data || T < 0 || (T > 0 && (!a_data || !out)) || N <= 0 || K <= 0 || (form != FP4_NV && form != FP4_MX) || K % fp4_block(form)) return -1;
   if ((reinterpret_cast<uintptr_t>(a_data) | reinterpret_cast<uintptr_t>(w_data)) & 15) return -1;
   if (pair && (N % 128 || residual)) return -1;
+  if (T > 65535 * 128) return -5;
   if (T == 0) return 0;
   if (x) {
     const int rc = ogb_quantize_fp4(x, ldx, x_fp32, T, K, form, a_data, stream);
     if (rc) return rc;
   }
-  Fp4LinearArgs p{fp4_view(a_data, T, K, form), fp4_view(const_cast<void*>(w_data), N, K, form), N, out, ldc, out_fp32, pair,
-                  static_cast<const __nv_bfloat16*>(bias), residual, ldr, res_fp32};
-  const dim3 grid(unsigned(((pair ? N / 2 : N) + TILE - 1) / TILE), unsigned((T + TILE - 1) / TILE));
+  static const int pdl = [] { const char* e = getenv("OGB_PDL"); return (e && e[0] == '0') ? 0 : 1; }();
+  Fp4LinearArgs p = {};
+  p.a = fp4_view(a_data, T, K, form);
+  p.w = fp4_view(const_cast<void*>(w_data), N, K, form);
+  p.N = N;
+  p.n_out = pair ? N / 2 : N;
+  p.C = out;
+  p.ldc = ldc;
+  p.out_fp32 = out_fp32;
+  p.pair = pair;
+  p.bias = static_cast<const __nv_bfloat16*>(bias);
+  p.residual = residual;
+  p.ldr = ldr;
+  p.res_fp32 = res_fp32;
+  p.whole = ((reinterpret_cast<uintptr_t>(out) | uintptr_t(ldc * (out_fp32 ? 4 : 2))) & 15) == 0 &&
+            (!residual || ((reinterpret_cast<uintptr_t>(residual) | uintptr_t(ldr * (res_fp32 ? 4 : 2))) & 15) == 0);
+  p.status = status;
+  p.pdl = pdl;
+  p.early = x != nullptr;      // the quantisation in front has waited for everything before it, and writes only the rows
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (form == FP4_NV) linear_fp4_simple_kernel<FP4_NV><<<grid, TILE * TILE, 0, s>>>(p); else linear_fp4_simple_kernel<FP4_MX><<<grid, TILE * TILE, 0, s>>>(p);
-  return cudaPeekAtLastError() == cudaSuccess ? 0 : -4;
+  return form == FP4_NV ? LaunchLinear<FP4_NV>(p, sm_count, s) : LaunchLinear<FP4_MX>(p, sm_count, s);
 }

@@ -40,6 +40,8 @@ __global__ void quantize_fp4_kernel(const T* x, long long ldx, int K, Fp4View ou
   __shared__ uint32_t s_top[32];
   const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* src = x + (long long)row * ldx;
+  pdl_wait();
+  pdl_launch_dependents();     // after the wait: whoever starts now may read what the kernels before this one wrote (linear_fp4.cu does)
   uint32_t top = 0;
   for (int k = threadIdx.x; k < K; k += blockDim.x) top = max(top, abs_bits(load_one(src + k)));
   top = __reduce_max_sync(0xffffffffu, top);
@@ -82,6 +84,8 @@ __global__ void quantize_fp4_kernel(const T* x, long long ldx, int K, Fp4View ou
 template <typename T, int FORM>
 __global__ void dequantize_fp4_kernel(Fp4View m, int K, T* out, long long ldo) {
   constexpr int B = FORM == FP4_NV ? 16 : 32;
+  pdl_wait();
+  pdl_launch_dependents();
   const int row = blockIdx.x;
   const float s = m.row_scale[row];
   for (int k = threadIdx.x; k < K; k += blockDim.x) {
@@ -109,14 +113,15 @@ OGB_API int ogb_quantize_fp4(const void* x, long long ldx, int x_fp32, int rows,
   if (rows == 0) return 0;
   const Fp4View v = fp4_view(data, rows, K, form);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  bool ok;
   if (x_fp32) {
-    if (form == FP4_NV) quantize_fp4_kernel<float, FP4_NV><<<rows, 256, 0, s>>>(static_cast<const float*>(x), ldx, K, v);
-    else quantize_fp4_kernel<float, FP4_MX><<<rows, 256, 0, s>>>(static_cast<const float*>(x), ldx, K, v);
+    ok = form == FP4_NV ? launch_pdl(quantize_fp4_kernel<float, FP4_NV>, dim3(rows), dim3(256), 0, s, static_cast<const float*>(x), ldx, K, v)
+                        : launch_pdl(quantize_fp4_kernel<float, FP4_MX>, dim3(rows), dim3(256), 0, s, static_cast<const float*>(x), ldx, K, v);
   } else {
-    if (form == FP4_NV) quantize_fp4_kernel<__nv_bfloat16, FP4_NV><<<rows, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ldx, K, v);
-    else quantize_fp4_kernel<__nv_bfloat16, FP4_MX><<<rows, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), ldx, K, v);
+    ok = form == FP4_NV ? launch_pdl(quantize_fp4_kernel<__nv_bfloat16, FP4_NV>, dim3(rows), dim3(256), 0, s, static_cast<const __nv_bfloat16*>(x), ldx, K, v)
+                        : launch_pdl(quantize_fp4_kernel<__nv_bfloat16, FP4_MX>, dim3(rows), dim3(256), 0, s, static_cast<const __nv_bfloat16*>(x), ldx, K, v);
   }
-  return cudaPeekAtLastError() == cudaSuccess ? 0 : -4;
+  return ok ? 0 : -4;
 }
 
 OGB_API int ogb_dequantize_fp4(const void* data, int rows, int K, int form, void* out, long long ldo, int out_fp32, void* stream) {

@@ -498,7 +498,7 @@ def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=N
         return y if out is None else out.copy_(y)
     if out is None:
         out = torch.empty(T, n_out, dtype=torch.float32 if out_fp32 else torch.bfloat16, device=w.device)
-    form = fp4_matrix.FORMS[w.form]
+    form, ws = fp4_matrix.FORMS[w.form], workspace(w.device)
     if given:
         rows, ldx, x32, a = None, 0, 0, x.data
     else:
@@ -509,7 +509,7 @@ def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=N
     with _on(w.device):
         _lib.check(_lib.lib().ogb_linear_fp4(rows, ldx, x32, a.data_ptr(), T, w.data.data_ptr(), N, K, form, out.data_ptr(), out.stride(0), int(out_fp32), int(pair),
                                              _ptr(bias), _ptr(residual), residual.stride(0) if residual is not None else 0,
-                                             int(residual is not None and residual.dtype == torch.float32), workspace(w.device).status, _stream()), "linear_fp4")
+                                             int(residual is not None and residual.dtype == torch.float32), ws.status, ws.sm_count, _stream()), "linear_fp4")
     return out
 
 

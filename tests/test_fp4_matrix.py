@@ -162,6 +162,6 @@ def test_launchers_refuse_on_the_host():
     assert L.ogb_quantize_fp4(None, 64, 0, 4, 64, 0, W, None) == -1
     assert L.ogb_quantize_fp4(A, 64, 0, 0, 64, 0, W, None) == 0           # nothing to do
     assert L.ogb_dequantize_fp4(W, 4, 64, 0, None, 64, 0, None) == -1
-    linear = lambda T=4, N=128, K=64, form=0, pair=0, res=None, w=W: L.ogb_linear_fp4(A, 64, 0, W, T, w, N, K, form, C, N, 0, pair, None, res, N, 0, None, None)
+    linear = lambda T=4, N=128, K=64, form=0, pair=0, res=None, w=W: L.ogb_linear_fp4(A, 64, 0, W, T, w, N, K, form, C, N, 0, pair, None, res, N, 0, None, 148, None)
     assert linear(T=-1) == -1 and linear(N=0) == -1 and linear(K=40) == -1 and linear(form=2) == -1 and linear(w=W + 4) == -1
     assert linear(N=64, pair=1) == -1 and linear(pair=1, res=C) == -1 and linear(T=0) == 0
