@@ -5,6 +5,8 @@
 // code, 0 where the block's scale is.  A power of two leaves x / s exact, so that no step before the last rounding moves a value across a tie.
 // mxfp4: a block's scale is 2^(floor(log2 max|block|) - 2), clamped to e8m0's range; an element's code is e2m1(x / scale), at most 6.  s = 1.
 // A row that holds an infinity or a NaN gets s = NaN, and everything computed from it is NaN.
+#include <cuda_fp16.h>
+
 #include "fp4_matrix.cuh"
 #include "kernels.h"
 
@@ -17,83 +19,211 @@ __device__ __forceinline__ int row_exponent(uint32_t top) {
   const int e = int(top >> 23) - 127;                       // max|x| = m 2^e, 1 <= m < 2; 2688 = 1.3125 * 2^11
   return max((top & 0x7fffffu) <= 0x280000u ? e - 11 : e - 10, -100);
 }
-__device__ __forceinline__ uint32_t e2m1_of(float q) {      // to nearest, ties to even, at most 6
-  const float a = fabsf(q);
-  const uint32_t c = (a > 0.25f) + (a >= 0.75f) + (a > 1.25f) + (a >= 1.75f) + (a > 2.5f) + (a >= 3.5f) + (a > 5.f);
-  return c | (q < 0.f && c ? 8u : 0u);
-}
 __device__ __forceinline__ uint32_t e4m3_of(float v) {      // 0 <= v <= 448, to nearest even
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
   return r & 0xffu;
 }
-
-template <typename T>
-__device__ __forceinline__ float load_one(const T* p) {
-  if constexpr (sizeof(T) == 4) return *p; else return bf2f(*p);
+// eight numbers to eight codes, the first in the lowest four bits: to nearest, ties to the even code, at most 6
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+      : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+__device__ __forceinline__ void values8(uint32_t codes, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(codes));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
-// One CTA per row; a thread takes whole blocks.
-template <typename T, int FORM>
-__global__ void quantize_fp4_kernel(const T* x, long long ldx, int K, Fp4View out) {
-  constexpr int B = FORM == FP4_NV ? 16 : 32;
-  __shared__ uint32_t s_top[32];
-  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* src = x + (long long)row * ldx;
+// Eight consecutive elements as they lie in memory.
+template <typename T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> {
+  uint4 q;
+  template <bool VEC> __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+    if constexpr (VEC) q = *reinterpret_cast<const uint4*>(p);
+    else {
+      const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+      q = make_uint4(u[0] | uint32_t(u[1]) << 16, u[2] | uint32_t(u[3]) << 16, u[4] | uint32_t(u[5]) << 16, u[6] | uint32_t(u[7]) << 16);
+    }
+  }
+  __device__ __forceinline__ void zero() { q = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  }
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+  template <bool VEC> __device__ __forceinline__ void load(const float* p) {
+    if constexpr (VEC) { a = reinterpret_cast<const float4*>(p)[0]; b = reinterpret_cast<const float4*>(p)[1]; }
+    else { a = make_float4(p[0], p[1], p[2], p[3]); b = make_float4(p[4], p[5], p[6], p[7]); }
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+};
+
+// A warp turns a row's k-blocks of 256, eight elements a lane: a block of 16 (32) belongs to two (four) lanes, the codes of a k-block go out as one
+// line of 128 bytes.  `wpr` warps share a row (a power of two, as many as it has k-blocks up to 16) and meet once, at the row's largest value; up to
+// QUANT_HELD k-blocks a warp stay in registers between the two passes, later ones are read again.
+constexpr int QUANT_HELD = 4;
+template <typename T, int FORM, bool VEC>
+__global__ void __launch_bounds__(512) quantize_fp4_kernel(const T* __restrict__ x, long long ldx, int K, int wpr, Fp4View out) {
+  __shared__ uint32_t s_top[16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp & (wpr - 1);
+  const int row = blockIdx.x * (int(blockDim.x >> 5) / wpr) + warp / wpr;
+  const bool here = row < out.rows;
+  const T* src = x + (long long)(here ? row : 0) * ldx;
   pdl_wait();
   pdl_launch_dependents();     // after the wait: whoever starts now may read what the kernels before this one wrote (linear_fp4.cu does)
+  Raw8<T> held[QUANT_HELD];
   uint32_t top = 0;
-  for (int k = threadIdx.x; k < K; k += blockDim.x) top = max(top, abs_bits(load_one(src + k)));
+  auto fetch = [&](int kb) {
+    Raw8<T> r;
+    const int k = kb * FP4_KB + lane * 8;
+    if (here && k < K) r.template load<VEC>(src + k); else r.zero();        // K is a multiple of 16: all eight or none
+    return r;
+  };
+  auto largest = [&](const Raw8<T>& r) {
+    float v[8];
+    r.get(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
+  };
+#pragma unroll
+  for (int i = 0; i < QUANT_HELD; ++i) held[i] = fetch(first + i * wpr);
+#pragma unroll
+  for (int i = 0; i < QUANT_HELD; ++i) largest(held[i]);
+  for (int kb = first + QUANT_HELD * wpr; kb < out.num_kb; kb += wpr) largest(fetch(kb));
   top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) s_top[warp] = top;
-  __syncthreads();
-  for (int w = 0; w < int(blockDim.x >> 5); ++w) top = max(top, s_top[w]);
+  if (wpr > 1) {
+    if (lane == 0) s_top[warp] = top;
+    __syncthreads();
+    for (int w = 0; w < wpr; ++w) top = max(top, s_top[(warp & ~(wpr - 1)) + w]);
+  }
+  if (!here) return;
   const bool bad = top >= 0x7f800000u;
   const int re = FORM == FP4_NV ? row_exponent(top) : 0;
-  if (threadIdx.x == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : pow2(re);
-  const float over = bad ? 0.f : pow2(-re);
-  for (int b = threadIdx.x; b < out.num_kb * (FP4_KB / B); b += blockDim.x) {
-    float v[B];
+  if (first == 0 && lane == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : pow2(re);
+  const float over = pow2(-re);
+
+  auto emit = [&](const Raw8<T>& r, int kb) {
+    float v[8];
     uint32_t m = 0;
-    for (int i = 0; i < B; ++i) {
-      const int k = b * B + i;
-      v[i] = k < K && !bad ? load_one(src + k) * over : 0.f;
-      m = max(m, abs_bits(v[i]));
+    r.get(v);
+    if (FORM == FP4_NV) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= over;
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     uint32_t code;
     if (FORM == FP4_NV) {
-      code = e4m3_of(__fdiv_rn(__uint_as_float(m), 6.f));
-      const float sc = fp4_scale_nv(code);
-      for (int i = 0; i < B; ++i) v[i] = code ? __fdiv_rn(v[i], sc) : 0.f;
+      code = bad ? 0u : e4m3_of(__fdiv_rn(__uint_as_float(m), 6.f));
+      const float sc = fp4_scale_nv(code), inv = code ? __frcp_rn(sc) : 0.f;
+      // v / sc: a product with the rounded reciprocal and one correction by the exact remainder, so that a quotient that is a tie comes out as that tie
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q = v[i] * inv;
+        v[i] = fmaf(fmaf(-q, sc, v[i]), inv, q);
+      }
     } else {
-      const float top_v = __uint_as_float(m);
-      int e = m >= 0x00800000u ? int(m >> 23) - 127 : (m ? ilogbf(top_v) : -127);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      int e = int(m >> 23) - 127;
+      if (m < 0x00800000u) e = m ? -118 - __clz(m) : -127;                 // below the normal numbers: m 2^-149
       e = max(e - 2, -127);
-      code = uint32_t(e + 127);
-      for (int i = 0; i < B; ++i) v[i] *= pow2(-e);
+      code = bad ? 0u : uint32_t(e + 127);
+      const float inv = pow2(-e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= inv;
     }
-    const int kb = b / (FP4_KB / B), in = b % (FP4_KB / B);
-    out.scales[fp4_scale_at(out, FORM, kb, row, in >> 2, in & 3)] = uint8_t(code);
-    for (int i = 0; i < B; i += 2) {
-      const int k = in * B + i;
-      out.codes[fp4_code_at(out, kb, row, k >> 5) + ((k & 31) >> 1)] = uint8_t(e2m1_of(v[i]) | (e2m1_of(v[i + 1]) << 4));
+    const uint32_t codes = bad ? 0u : e2m1x8(v);
+    *reinterpret_cast<uint32_t*>(out.codes + fp4_code_at(out, kb, row, lane >> 2) + (lane & 3) * 4) = codes;
+    constexpr int PER = FORM == FP4_NV ? 2 : 4;                              // lanes of a block; four blocks' scales are one word
+    const uint32_t c1 = __shfl_down_sync(0xffffffffu, code, PER), c2 = __shfl_down_sync(0xffffffffu, code, 2 * PER), c3 = __shfl_down_sync(0xffffffffu, code, 3 * PER);
+    if (lane % (4 * PER) == 0)
+      *reinterpret_cast<uint32_t*>(out.scales + fp4_scale_at(out, FORM, kb, row, lane / (4 * PER), 0)) = code | c1 << 8 | c2 << 16 | c3 << 24;
+  };
+#pragma unroll
+  for (int i = 0; i < QUANT_HELD; ++i)
+    if (first + i * wpr < out.num_kb) emit(held[i], first + i * wpr);
+  for (int kb = first + QUANT_HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb), kb);
+}
+
+// A warp reads four rows of a k-block (512 bytes of codes), eight elements a lane and row.
+constexpr int DEQUANT_ROWS = 4;
+template <typename T, int FORM>
+__global__ void __launch_bounds__(256) dequantize_fp4_kernel(Fp4View m, int K, T* __restrict__ out, long long ldo, int vec) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, row0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * DEQUANT_ROWS, kb = blockIdx.y;
+  const int k = kb * FP4_KB + lane * 8, b = lane / (FORM == FP4_NV ? 2 : 4);
+  if (k >= K) return;
+  uint32_t codes[DEQUANT_ROWS];
+  float scale[DEQUANT_ROWS];
+#pragma unroll
+  for (int i = 0; i < DEQUANT_ROWS; ++i) {
+    const int r = min(row0 + i, m.rows - 1);
+    codes[i] = *reinterpret_cast<const uint32_t*>(m.codes + fp4_code_at(m, kb, r, lane >> 2) + (lane & 3) * 4);
+    scale[i] = fp4_scale(FORM, m.scales[fp4_scale_at(m, FORM, kb, r, b >> 2, b & 3)]) * m.row_scale[r];
+  }
+#pragma unroll
+  for (int i = 0; i < DEQUANT_ROWS; ++i) {
+    if (row0 + i >= m.rows) break;
+    float v[8];
+    values8(codes[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= scale[i];
+    T* dst = out + (long long)(row0 + i) * ldo + k;
+    if constexpr (sizeof(T) == 4) {
+      if (vec) { reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]); reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]); }
+      else for (int j = 0; j < 8; ++j) dst[j] = v[j];
+    } else {
+      if (vec) *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+      else for (int j = 0; j < 8; ++j) dst[j] = f2bf(v[j]);
     }
   }
 }
 
 template <typename T, int FORM>
-__global__ void dequantize_fp4_kernel(Fp4View m, int K, T* out, long long ldo) {
-  constexpr int B = FORM == FP4_NV ? 16 : 32;
-  pdl_wait();
-  pdl_launch_dependents();
-  const int row = blockIdx.x;
-  const float s = m.row_scale[row];
-  for (int k = threadIdx.x; k < K; k += blockDim.x) {
-    const int kb = k / FP4_KB, in = k % FP4_KB, b = in / B;
-    const uint32_t byte = m.codes[fp4_code_at(m, kb, row, in >> 5) + ((in & 31) >> 1)];
-    const float v = fp4_value((in & 1) ? byte >> 4 : byte & 15u) * fp4_scale(FORM, m.scales[fp4_scale_at(m, FORM, kb, row, b >> 2, b & 3)]) * s;
-    if constexpr (sizeof(T) == 4) out[(long long)row * ldo + k] = v; else out[(long long)row * ldo + k] = f2bf(v);
-  }
+static bool LaunchQuantize(const void* x, long long ldx, int K, const Fp4View& v, cudaStream_t s) {
+  int wpr = 1;
+  while (wpr < v.num_kb && wpr < 16) wpr *= 2;
+  const int warps = wpr == 16 ? 16 : 8, rows_per_cta = warps / wpr;
+  const dim3 grid(unsigned((v.rows + rows_per_cta - 1) / rows_per_cta)), block(unsigned(warps * 32));
+  const T* p = static_cast<const T*>(x);
+  const bool vec = ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * (long long)sizeof(T))) & 15) == 0;
+  return vec ? launch_pdl(quantize_fp4_kernel<T, FORM, true>, grid, block, 0, s, p, ldx, K, wpr, v)
+             : launch_pdl(quantize_fp4_kernel<T, FORM, false>, grid, block, 0, s, p, ldx, K, wpr, v);
+}
+template <typename T>
+static bool LaunchDequantize(const Fp4View& v, int K, int form, void* out, long long ldo, cudaStream_t s) {
+  const dim3 grid(unsigned((v.rows + 8 * DEQUANT_ROWS - 1) / (8 * DEQUANT_ROWS)), unsigned(v.num_kb));
+  T* p = static_cast<T*>(out);
+  const int vec = ((reinterpret_cast<uintptr_t>(out) | uintptr_t(ldo * (long long)sizeof(T))) & 15) == 0;
+  return form == FP4_NV ? launch_pdl(dequantize_fp4_kernel<T, FP4_NV>, grid, dim3(256), 0, s, v, K, p, ldo, vec)
+                        : launch_pdl(dequantize_fp4_kernel<T, FP4_MX>, grid, dim3(256), 0, s, v, K, p, ldo, vec);
 }
 
 }  // namespace ogb
@@ -113,14 +243,8 @@ OGB_API int ogb_quantize_fp4(const void* x, long long ldx, int x_fp32, int rows,
   if (rows == 0) return 0;
   const Fp4View v = fp4_view(data, rows, K, form);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  bool ok;
-  if (x_fp32) {
-    ok = form == FP4_NV ? launch_pdl(quantize_fp4_kernel<float, FP4_NV>, dim3(rows), dim3(256), 0, s, static_cast<const float*>(x), ldx, K, v)
-                        : launch_pdl(quantize_fp4_kernel<float, FP4_MX>, dim3(rows), dim3(256), 0, s, static_cast<const float*>(x), ldx, K, v);
-  } else {
-    ok = form == FP4_NV ? launch_pdl(quantize_fp4_kernel<__nv_bfloat16, FP4_NV>, dim3(rows), dim3(256), 0, s, static_cast<const __nv_bfloat16*>(x), ldx, K, v)
-                        : launch_pdl(quantize_fp4_kernel<__nv_bfloat16, FP4_MX>, dim3(rows), dim3(256), 0, s, static_cast<const __nv_bfloat16*>(x), ldx, K, v);
-  }
+  const bool ok = x_fp32 ? (form == FP4_NV ? LaunchQuantize<float, FP4_NV>(x, ldx, K, v, s) : LaunchQuantize<float, FP4_MX>(x, ldx, K, v, s))
+                         : (form == FP4_NV ? LaunchQuantize<__nv_bfloat16, FP4_NV>(x, ldx, K, v, s) : LaunchQuantize<__nv_bfloat16, FP4_MX>(x, ldx, K, v, s));
   return ok ? 0 : -4;
 }
 
@@ -129,12 +253,6 @@ OGB_API int ogb_dequantize_fp4(const void* data, int rows, int K, int form, void
   if (rows == 0) return 0;
   const Fp4View v = fp4_view(const_cast<void*>(data), rows, K, form);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (out_fp32) {
-    if (form == FP4_NV) dequantize_fp4_kernel<float, FP4_NV><<<rows, 256, 0, s>>>(v, K, static_cast<float*>(out), ldo);
-    else dequantize_fp4_kernel<float, FP4_MX><<<rows, 256, 0, s>>>(v, K, static_cast<float*>(out), ldo);
-  } else {
-    if (form == FP4_NV) dequantize_fp4_kernel<__nv_bfloat16, FP4_NV><<<rows, 256, 0, s>>>(v, K, static_cast<__nv_bfloat16*>(out), ldo);
-    else dequantize_fp4_kernel<__nv_bfloat16, FP4_MX><<<rows, 256, 0, s>>>(v, K, static_cast<__nv_bfloat16*>(out), ldo);
-  }
-  return cudaPeekAtLastError() == cudaSuccess ? 0 : -4;
+  if (v.num_kb > 65535) return -5;
+  return (out_fp32 ? LaunchDequantize<float>(v, K, form, out, ldo, s) : LaunchDequantize<__nv_bfloat16>(v, K, form, out, ldo, s)) ? 0 : -4;
 }
