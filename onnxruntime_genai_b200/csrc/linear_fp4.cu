@@ -24,7 +24,8 @@ struct Fp4LinearArgs {
   long long ldr;
   int res_fp32;
   int whole;                    // every eight columns of an output and residual row are aligned for 16-byte accesses
-  int splits, kb_per_split;
+  int splits, kb_per_split;     // parts of the k-blocks, none of them empty
+  int stages;
   int early;                    // weights may be fetched before the kernel in front has finished (it does not write them, nor do those before it)
   int* status;
   int pdl;
@@ -112,35 +113,44 @@ struct Fp4Cfg {
   static constexpr int SF = fp4_sf_bytes(FORM);
   static constexpr int X_OFF = FP4_W_BYTES, SFW_OFF = X_OFF + BT * 128, SFX_OFF = SFW_OFF + SF;
   static constexpr int STAGE = SFX_OFF + SF;                                     // codes of weights and tokens, scales of weights and of 128 tokens
-  static constexpr int STAGES = 110 * 1024 / STAGE < 8 ? 110 * 1024 / STAGE : 8;  // two CTAs per SM
+  // Partial sums that other CTAs of the cluster send: up to 32 tokens have a place of their own, more take the stages once the whole cluster is done with them
+  static constexpr bool APART = BT <= 32;
+  static constexpr int SUMS = (BT + 8) * FP4_TILE * 4;
+  static constexpr int STAGES = (110 * 1024 - (APART ? SUMS : 0)) / STAGE;         // two CTAs per SM
   static constexpr int SF_COL = BT < 32 ? 32 : BT;                                // first tensor-memory column of the scales: two sets of 16 + 16
   static constexpr int COLS = SF_COL + 64 <= 128 ? 128 : 256;
-  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;
-  static_assert(STAGE % 1024 == 0 && BT * FP4_TILE * 4 <= STAGES * STAGE && 2 * (SMEM + 1024) <= 228 * 1024, "shared memory");
+  static_assert(STAGE % 1024 == 0 && STAGES >= 2, "stages");
+  static constexpr int smem(int stages) {
+    const int ring = stages * STAGE;
+    return (APART ? ring + SUMS : ring > SUMS ? ring : SUMS) + 1024 + 256;
+  }
 };
 
 template <int BT, int FORM>
-__global__ void __launch_bounds__(192, 2) linear_fp4_kernel(const Fp4LinearArgs p) {
+__global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs p) {
   using Cfg = Fp4Cfg<BT, FORM>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::STAGES * Cfg::STAGE);
+  const int stages = p.stages, ring = stages * Cfg::STAGE;
+  float* sums = reinterpret_cast<float*>(smem + (Cfg::APART ? ring : 0));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Cfg::smem(stages) - 1024 - 256);
   uint64_t* empty = full + Cfg::STAGES;
   uint64_t* accum = empty + Cfg::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int n_tile = blockIdx.x, row0 = blockIdx.y * BT, rows = min(BT, p.a.rows - row0);
-  const int kb0 = blockIdx.z * p.kb_per_split, num = max(0, min(p.kb_per_split, p.w.num_kb - kb0));
+  const int kb0 = blockIdx.z * p.kb_per_split, num = min(p.kb_per_split, p.w.num_kb - kb0);       // at least one
   auto fail = [&](int code) { atomicMax(p.status, code); *abort_flag = 1; };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < Cfg::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < stages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     mbar_init(accum, 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 1) { tmem_alloc(tmem_slot, Cfg::COLS); tmem_relinquish(); }
+  if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");         // sums are sent to CTAs that run
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -166,7 +176,7 @@ __global__ void __launch_bounds__(192, 2) linear_fp4_kernel(const Fp4LinearArgs 
       bulk_copy_g2s(st + Cfg::X_OFF, x + (kb0 + i) * x_step, BT * 128, &full[s]);
       bulk_copy_g2s(st + Cfg::SFX_OFF, sx + (kb0 + i) * sx_step, Cfg::SF, &full[s]);
     };
-    const int ahead = min(num, Cfg::STAGES);
+    const int ahead = min(num, stages);
     if (p.pdl && !p.early) pdl_wait();
     if (elect_one()) for (int i = 0; i < ahead; ++i) weights(i, i);
     __syncwarp();
@@ -182,11 +192,11 @@ __global__ void __launch_bounds__(192, 2) linear_fp4_kernel(const Fp4LinearArgs 
       if (elect_one()) { weights(i, s); tokens(i, s); }
       __syncwarp();
       ++filled;
-      if (++s == Cfg::STAGES) { s = 0; ph ^= 1; }
+      if (++s == stages) { s = 0; ph ^= 1; }
     }
     if (!ok || *abort_flag) {     // copies in flight still write this shared memory: give them time to land
       volatile int never = 0;
-      for (int i = max(0, filled - Cfg::STAGES); i < filled; ++i) mbar_wait_bounded(&full[i % Cfg::STAGES], (i / Cfg::STAGES) & 1, &never, 200000000ull);
+      for (int i = max(0, filled - stages); i < filled; ++i) mbar_wait_bounded(&full[i % stages], (i / stages) & 1, &never, 200000000ull);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products
@@ -214,72 +224,89 @@ __global__ void __launch_bounds__(192, 2) linear_fp4_kernel(const Fp4LinearArgs 
         if (i == num - 1) umma_commit(accum);
       }
       __syncwarp();
-      if (++s == Cfg::STAGES) { s = 0; ph ^= 1; }
+      if (++s == stages) { s = 0; ph ^= 1; }
     }
   }
-  // ------------------------------------------------------------------ accumulators to shared memory, sums over the cluster, results (warps 2..5)
-  float* part = reinterpret_cast<float*>(smem);               // [BT][128] in the stages: all copies and products are done when the accumulator is
-  const int et = int(threadIdx.x) - 64;
+
+  // ------------------------------------------------------------------ results (warps 2..5)
+  // Token rows are dealt out to the CTAs of the cluster; every CTA sends its part of a row's sums to the row's CTA, at [sender][row][128 outputs].
+  const int rank = p.splits > 1 ? int(cluster_ctarank()) : 0, per = (rows + p.splits - 1) / p.splits;
+  const int et = int(threadIdx.x) - 64, segs = p.pair ? 8 : 16, seg = (et & (segs - 1)) * 8, g = n_tile * FP4_TILE + seg;
+  const int first = min(rows, rank * per), last = min(rows, first + per);
+  float ws[8], us[8], wb[8], ub[8];
   if (warp >= 2) {
-    const int quarter = warp & 3, row = quarter * 32 + lane;
-    if (num > 0) {
-      if (!mbar_wait_bounded(accum, 0, abort_flag, 4000000000ull)) fail(OGB_ERR_WAIT_MMA);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (*abort_flag == 0) {
-        tc_fence_after();
-#pragma unroll 1
-        for (int c0 = 0; c0 < BT && c0 < rows; c0 += 16) {
-          uint32_t r[16];
-          tmem_ld16(tmem + (uint32_t(quarter * 32) << 16) + c0, r);
-          tmem_ld_wait();
+    if (p.pdl) pdl_wait();
+    if (first < last) {                       // row scales and bias of this thread's columns, fetched under the main loop
 #pragma unroll
-          for (int j = 0; j < 16; ++j) part[(c0 + j) * FP4_TILE + row] = __uint_as_float(r[j]);
-        }
+      for (int j = 0; j < 8; ++j) {
+        ws[j] = p.w.row_scale[g + j];
+        wb[j] = p.bias && g + j < p.N ? bf2f(p.bias[g + j]) : 0.f;
+        us[j] = p.pair ? p.w.row_scale[g + 64 + j] : 0.f;
+        ub[j] = p.pair && p.bias ? bf2f(p.bias[g + 64 + j]) : 0.f;
       }
     }
-    if (p.pdl) pdl_wait();
+    if (!mbar_wait_bounded(accum, 0, abort_flag, 4000000000ull)) fail(OGB_ERR_WAIT_MMA);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    tc_fence_after();
+  }
+  __syncwarp();
+  if (p.splits > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");                            // of the arrival at the start
+    if (!Cfg::APART) cluster_sync_all();                                                // nobody's stages are in use any more
+  }
+  if (warp >= 2 && *abort_flag == 0) {
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t at = smem_u32(sums);
+#pragma unroll 1
+    for (int c0 = 0; c0 < rows; c0 += 16) {
+      uint32_t r[16];
+      tmem_ld16(tmem + (uint32_t(quarter * 32) << 16) + c0, r);
+      tmem_ld_wait();
+      if (p.splits > 1) {
+        int m = c0, o = c0 / per, l = c0 - o * per;                                       // token, its CTA and its place there
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (m < rows) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dsmem_addr(at + uint32_t((rank * per + l) * FP4_TILE + row) * 4, uint32_t(o))), "r"(r[j]) : "memory");
+          ++m;
+          if (++l == per) { l = 0; ++o; }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sums[(c0 + j) * FP4_TILE + row] = __uint_as_float(r[j]);
+      }
+    }
   }
   __syncwarp();
   tc_fence_before();
   if (p.splits > 1) cluster_sync_all(); else __syncthreads();
   if (warp >= 2 && *abort_flag == 0) {
-    const int rank = p.splits > 1 ? int(cluster_ctarank()) : 0;
-    const int per = (rows + p.splits - 1) / p.splits, first = min(rows, rank * per), last = min(rows, first + per);   // tokens that this CTA finishes
-    const int segs = p.pair ? 8 : 16, used = min(p.splits, (p.w.num_kb + p.kb_per_split - 1) / p.kb_per_split);
-    const uint32_t at = smem_u32(part);
-    auto sum8 = [&](int m, int n, float scale, float (&v)[8]) {
+    const int col = n_tile * (p.pair ? 64 : 128) + seg;
+    if (col < p.n_out) {
+      for (int m = first + (p.pair ? et >> 3 : et >> 4); m < last; m += 128 / segs) {
+        const float scale = p.a.row_scale[row0 + m];
+        float v[8], u[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      for (int q = 0; q < used; ++q) {
-        const uint32_t a = p.splits > 1 ? dsmem_addr(at + uint32_t(m * FP4_TILE + n) * 4, uint32_t(q)) : 0u;
-        const float4* l = reinterpret_cast<const float4*>(part + m * FP4_TILE + n);
-        const float4 x = p.splits > 1 ? ld_dsmem_f32x4(a) : l[0], y = p.splits > 1 ? ld_dsmem_f32x4(a + 16) : l[1];
-        v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
-      }
-      const int g = n_tile * FP4_TILE + n;                     // (row scales are padded to whole tiles)
+        for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
+        for (int q = 0; q < p.splits; ++q) {
+          const float4* l = reinterpret_cast<const float4*>(sums + (q * per + m - first) * FP4_TILE + seg);
+          const float4 x = l[0], y = l[1];
+          v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w; v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+          if (p.pair) {
+            const float4 a = l[16], b = l[17];
+            u[0] += a.x; u[1] += a.y; u[2] += a.z; u[3] += a.w; u[4] += b.x; u[5] += b.y; u[6] += b.z; u[7] += b.w;
+          }
+        }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] *= scale * p.w.row_scale[g + j];
-        if (p.bias && g + j < p.N) v[j] += bf2f(p.bias[g + j]);
-      }
-    };
-    for (int i = et; i < (last - first) * segs; i += 128) {
-      const int m = first + i / segs, seg = i % segs * 8, col = n_tile * (p.pair ? 64 : 128) + seg;
-      if (col >= p.n_out) continue;
-      const float scale = p.a.row_scale[row0 + m];
-      float v[8];
-      sum8(m, seg, scale, v);
-      if (p.pair) {
-        float u[8];
-        sum8(m, seg + 64, scale, u);
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], scale * ws[j], wb[j]);
+        if (p.pair) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = silu(v[j]) * u[j];
+          for (int j = 0; j < 8; ++j) v[j] = silu(v[j]) * fmaf(u[j], scale * us[j], ub[j]);
+        }
+        fp4_store8(p, row0 + m, col, v);
       }
-      fp4_store8(p, row0 + m, col, v);
     }
   }
-  __syncwarp();
-  if (p.splits > 1) cluster_sync_all(); else __syncthreads();   // no CTA leaves while another reads its sums
+  __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, Cfg::COLS);
 }
 
@@ -287,13 +314,14 @@ template <int BT, int FORM>
 static int LaunchFew(Fp4LinearArgs p, int splits, cudaStream_t stream) {
   using Cfg = Fp4Cfg<BT, FORM>;
   static bool configured[OGB_MAX_DEVICES] = {};
-  if (!set_max_dyn_smem(linear_fp4_kernel<BT, FORM>, Cfg::SMEM, configured)) return -3;
-  p.splits = splits;
+  if (!set_max_dyn_smem(linear_fp4_kernel<BT, FORM>, Cfg::smem(Cfg::STAGES), configured)) return -3;
   p.kb_per_split = (p.w.num_kb + splits - 1) / splits;
+  p.splits = splits = (p.w.num_kb + p.kb_per_split - 1) / p.kb_per_split;
+  p.stages = min(Cfg::STAGES, p.kb_per_split);       // no more shared memory than the CTA has k-blocks: the next kernel's CTAs find room
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(p.w.padded / FP4_TILE), unsigned((p.a.rows + BT - 1) / BT), unsigned(splits));
   cfg.blockDim = dim3(192);
-  cfg.dynamicSmemBytes = Cfg::SMEM;
+  cfg.dynamicSmemBytes = Cfg::smem(p.stages);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   int n = 0;

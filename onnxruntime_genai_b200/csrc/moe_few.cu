@@ -52,7 +52,6 @@ struct FewArgs {
   float alpha, limit;
   FewPlan* plan;
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
-  int x_vec;            // rows of x are aligned for 16-byte loads
 };
 
 // ------------------------------------------------------------------------------- operands
@@ -191,47 +190,53 @@ __device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // 
 // Shared memory of the first kernel.
 struct FewShared {
   float red[8][16 * FEW_TOKENS];
-  float unscale[FEW_TOKENS];
+  uint32_t top[FEW_TOKENS];          // bits of the rows' largest magnitudes
   uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
   FewPlan plan;
 };
 
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int vec) {
-  if (vec) return *reinterpret_cast<const uint4*>(p);
-  const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-  return make_uint4(u[0] | uint32_t(u[1]) << 16, u[2] | uint32_t(u[3]) << 16, u[4] | uint32_t(u[5]) << 16, u[6] | uint32_t(u[7]) << 16);
+// Power of two that brings a row's largest magnitude (its bits) to 2^14 .. 2^15
+__device__ __forceinline__ int few_shift(uint32_t top) { return top >= 0x7f800000u ? 0 : min(14 - (int(top >> 23) - 127), 126); }
+// A float as an unsigned number of the same order; 0: not a number.
+__device__ __forceinline__ uint32_t few_key(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return v != v ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-
-// Choice of `top` experts for a token by one warp: the largest logits, the lowest index among equal ones; a token whose logits are not numbers takes expert 0.
+// Choice of `top` experts for a token by one warp: the largest logits, the lowest index among equal ones; a token whose logits are not numbers takes
+// expert 0.  A lane holds every 32nd expert and looks for its best one anew only when that was taken.
 __device__ __forceinline__ void few_choose(const float* row, int E, int top, int rule, int lane, int& id, float& share) {
-  uint32_t taken = 0;                // bit i: expert lane + 32 i
-  float most = -INFINITY, all = 0.f;
+  uint32_t taken = 0, best = 0;      // taken, bit i: expert lane + 32 i
+  int at = 0x7fffffff;
   bool bad = false;
-  for (int e = lane; e < E; e += 32) { most = fmaxf(most, row[e]); bad |= row[e] != row[e]; }
-  most = warp_max(most);
+  auto scan = [&]() {
+    best = 0;
+    at = 0x7fffffff;
+    for (int i = 0, e = lane; e < E; ++i, e += 32) {
+      const uint32_t k = taken >> i & 1 ? 0u : few_key(row[e]);
+      if (k > best) { best = k; at = e; }
+    }
+  };
+  for (int e = lane; e < E; e += 32) bad |= row[e] != row[e];
   bad = __any_sync(0xffffffffu, bad);
-  if (rule == 1) {
-    for (int e = lane; e < E; e += 32) all += expf(row[e] - most);
-    all = warp_sum(all);
-  }
-  float mine = -INFINITY;
+  scan();
+  float most = 0.f, mine = 0.f;
   id = 0;
   for (int j = 0; j < top; ++j) {
-    float best = -INFINITY;
-    int at = 0x7fffffff;
-    for (int i = 0, e = lane; e < E; ++i, e += 32)
-      if (!(taken >> i & 1) && (row[e] > best || (row[e] == best && e < at))) { best = row[e]; at = e; }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-      if (ov > best || (ov == best && oa < at)) { best = ov; at = oa; }
-    }
-    if (at != 0x7fffffff && (at & 31) == lane) taken |= 1u << (at >> 5);
-    if (lane == j) { mine = best; id = at == 0x7fffffff ? 0 : at; }
+    const uint32_t k = __reduce_max_sync(0xffffffffu, best);
+    const int e = int(__reduce_min_sync(0xffffffffu, best == k && k ? uint32_t(at) : 0x7fffffffu));
+    const float v = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    if (j == 0) most = v;
+    if (lane == j) { mine = v; id = k ? e : 0; }
+    if (k && at == e) { taken |= 1u << (e >> 5); scan(); }
   }
-  const float w = lane < top ? expf(mine - most) : 0.f, sum = warp_sum(w);
-  share = bad ? __uint_as_float(0x7fc00000u) : w / (rule == 1 ? all : sum);
+  const float w = lane < top ? expf(mine - most) : 0.f;
+  float sum = warp_sum(w);
+  if (rule == 1) {
+    sum = 0.f;
+    for (int e = lane; e < E; e += 32) sum += expf(row[e] - most);
+    sum = warp_sum(sum);
+  }
+  share = bad ? __uint_as_float(0x7fc00000u) : w / sum;
 }
 
 template <int W>
@@ -246,34 +251,24 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
   const int rank = int(cluster_ctarank());
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the others' shared memory is written only once they run
   for (int e = threadIdx.x; e < p.E; e += FEW_A_THREADS) sh.mask[e] = 0;
+  if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
+  __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
 
-  // the rows, as the products read them: a warp per token
-  if (warp < p.T) {
-    const __nv_bfloat16* src = p.x + warp * p.ldx;
-    float scale = 1.f;
-    if (W == FEW_FP4_F16) {
+  // the largest magnitude of every row, where the rows are to be scaled: a warp takes 256 values of a token at a time
+  const int parts = (Hp + 255) >> 8, pieces = p.T * parts;
+  if (W == FEW_FP4_F16) {
+#pragma unroll 4
+    for (int i = warp; i < pieces; i += 8) {
+      const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
+      const uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       uint32_t top = 0;
-      for (int k = lane * 8; k < p.H; k += 256) {
-        const uint4 v = load8(src + k, p.x_vec);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, max(w[i] << 16 & 0x7fffffffu, w[i] & 0x7fff0000u));
-      }
+      for (int j = 0; j < 4; ++j) top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
       top = __reduce_max_sync(0xffffffffu, top);
-      const int k = top >= 0x7f800000u ? 0 : min(14 - (int(top >> 23) - 127), 126);       // the largest value to 2^14 .. 2^15
-      scale = __uint_as_float(uint32_t(k + 127) << 23);
-      if (lane == 0) sh.unscale[warp] = __uint_as_float(uint32_t(127 - k) << 23);
-    }
-    for (int k = lane * 8; k < Hp; k += 256) {
-      uint4 v = k < p.H ? load8(src + k, p.x_vec) : make_uint4(0, 0, 0, 0);
-      if (W == FEW_FP4_F16) {
-        const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
-        v = make_uint4(pack_f16x2(a.x * scale, c.x * scale), pack_f16x2(a.y * scale, c.y * scale), pack_f16x2(b.x * scale, d.x * scale),
-                       pack_f16x2(b.y * scale, d.y * scale));
-      }
-      *reinterpret_cast<uint4*>(xs + warp * xs_ld + k) = v;
+      if (lane == 0) atomicMax(&sh.top[t], top);
     }
   }
 
@@ -290,7 +285,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
     for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += 256) {
       const bool in = k < p.H;
       const uint4 a0 = r0 && in ? *reinterpret_cast<const uint4*>(w0 + k) : zero, a1 = r1 && in ? *reinterpret_cast<const uint4*>(w1 + k) : zero;
-      const uint4 b = g < p.T && in ? load8(p.x + g * p.ldx + k, p.x_vec) : zero;
+      const uint4 b = g < p.T && in ? *reinterpret_cast<const uint4*>(p.x + g * p.ldx + k) : zero;
       mma_bf16_32(acc, a0, a1, b);
     }
     *reinterpret_cast<float2*>(&sh.red[warp][g * 8 + q * 2]) = make_float2(acc[0], acc[1]);
@@ -311,7 +306,21 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
     }
     __syncthreads();
   }
-  cluster_sync_all();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  // the rows as the products read them
+#pragma unroll 4
+  for (int i = warp; i < pieces; i += 8) {
+    const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
+    uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+    if (W == FEW_FP4_F16) {
+      const float scale = __uint_as_float(uint32_t(few_shift(sh.top[t]) + 127) << 23);
+      const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
+      v = make_uint4(pack_f16x2(a.x * scale, c.x * scale), pack_f16x2(a.y * scale, c.y * scale), pack_f16x2(b.x * scale, d.x * scale),
+                     pack_f16x2(b.y * scale, d.y * scale));
+    }
+    if (k < Hp) *reinterpret_cast<uint4*>(xs + t * xs_ld + k) = v;
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
   // choices, and the experts that any token meets
   if (warp < p.T) {
@@ -388,7 +397,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
       for (int j = 0; j < 2; ++j) {
         const int t = q * 2 + j, slot = sh.plan.slot[d][t];
         if (slot != 255) {
-          const float s = W == FEW_FP4_F16 ? sh.unscale[t] : 1.f;
+          const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) : 1.f;
           float gate = fmaf(acc[j], s, bg), up = fmaf(acc[2 + j], s, bu), v;
           if (p.act == 2) {
             if (p.limit > 0.f) {             // (comparisons, not minima: what is not a number stays that)
@@ -540,12 +549,11 @@ OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router,
                                float alpha, float limit, void* scratch, void* stream) {
   if (ogb_moe_few_scratch_bytes(T, top, I) < 0 || !x || !router || !gate_up || !down || !out || !scratch || H < 1 || H % 8 || E < top || E > FEW_EXPERTS ||
       I % 64 || (weights != FEW_BF16 && H % 64) || rule < 0 || rule > 2 || weights < 0 || weights > 2 || (act != 1 && act != 2)) return -1;
-  if ((reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(scratch)) & 15)
+  if ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * 2) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(scratch)) & 15)
     return -1;
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,
             static_cast<const __nv_bfloat16*>(gate_up_b), down, static_cast<const __nv_bfloat16*>(down_b), static_cast<__nv_bfloat16*>(out), T, H, I, E, top,
-            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)),
-            ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * 2)) & 15) == 0};
+            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan))};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, s);
   return weights == FEW_FP4_F16 ? LaunchFew<FEW_FP4_F16>(p, s) : LaunchFew<FEW_FP4_BF16>(p, s);

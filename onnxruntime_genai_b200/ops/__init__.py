@@ -435,9 +435,12 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     return _gemm(x, w, out, bias, residual, flags, splits, fused)
 
 
-def _on(device):
-    """The stream that a call on `device` uses: the current one of that device, made the current device for the call where it is another."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call_on(index: int, entry: str, *args):
+    """Runs an entry point of the kernel library on device `index`, on that device's current stream (the last argument)."""
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _call_on(index, entry, *args)
+    _lib.check(getattr(_lib.lib(), entry)(*args, torch._C._cuda_getCurrentRawStream(index)), entry)
 
 
 def quantize_fp4(x, form: str = "nvfp4") -> Fp4Matrix:
@@ -454,41 +457,41 @@ def quantize_fp4(x, form: str = "nvfp4") -> Fp4Matrix:
     if x.stride(1) != 1:
         x = x.contiguous()
     data = torch.empty(fp4_matrix.matrix_bytes(T, K, form), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        _lib.check(_lib.lib().ogb_quantize_fp4(x.data_ptr(), x.stride(0), int(x.dtype == torch.float32), T, K, fp4_matrix.FORMS[form], data.data_ptr(),
-                                               _stream()), "quantize_fp4")
+    _call_on(x.get_device(), "ogb_quantize_fp4", x.data_ptr(), x.stride(0), x.dtype == torch.float32, T, K, fp4_matrix.FORMS[form], data.data_ptr())
     return Fp4Matrix(data, T, K, form)
 
 
 def _dequantize_fp4(m: Fp4Matrix, dtype):
     out = torch.empty(m.rows, m.K, dtype=dtype, device=m.device)
-    with _on(m.device):
-        _lib.check(_lib.lib().ogb_dequantize_fp4(m.data.data_ptr(), m.rows, m.K, fp4_matrix.FORMS[m.form], out.data_ptr(), m.K, int(dtype == torch.float32),
-                                                 _stream()), "dequantize_fp4")
+    _call_on(m.data.get_device(), "ogb_dequantize_fp4", m.data.data_ptr(), m.rows, m.K, fp4_matrix.FORMS[m.form], out.data_ptr(), m.K, dtype == torch.float32)
     return out
 
 
 def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=None, pair=False):
     """The product of 4-bit rows and weights; x: rows still to be quantised, or an Fp4Matrix of w's form."""
-    N, K = w.shape
+    N, K, data, cuda = w.rows, w.K, w.data, w.data.is_cuda
     n_out = N // 2 if pair else N
     given = isinstance(x, Fp4Matrix)
-    if given and x.form != w.form:
-        raise ValueError(f"rows in {x.form} and weights in {w.form}")
-    if not given and (x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32)):
-        raise ValueError(f"rows [T, K] in bfloat16 or float32 are wanted, not {tuple(x.shape)} in {x.dtype}")
-    T = x.shape[0]
-    if x.shape[1] != K:
-        raise ValueError(f"rows of {x.shape[1]} and weights of {K}")
-    if x.device != w.device or any(t is not None and t.device != w.device for t in (bias, residual, out)):
+    if given:
+        if x.form != w.form:
+            raise ValueError(f"rows in {x.form} and weights in {w.form}")
+        T, Kx = x.rows, x.K
+    else:
+        if x.dim() != 2 or (x.dtype != torch.bfloat16 and x.dtype != torch.float32):
+            raise ValueError(f"rows [T, K] in bfloat16 or float32 are wanted, not {tuple(x.shape)} in {x.dtype}")
+        T, Kx = x.shape
+    if Kx != K:
+        raise ValueError(f"rows of {Kx} and weights of {K}")
+    dev = data.device
+    if x.device != dev or (bias is not None and bias.device != dev) or (residual is not None and residual.device != dev) or (out is not None and out.device != dev):
         raise ValueError("rows, weights, bias, residual and output are on different devices")
-    if bias is not None and (bias.shape != (N,) or (w.is_cuda and (bias.dtype != torch.bfloat16 or bias.stride(0) != 1))):
+    if bias is not None and (bias.shape != (N,) or (cuda and (bias.dtype != torch.bfloat16 or bias.stride(0) != 1))):
         raise ValueError(f"the bias of {N} outputs is bfloat16 [{N}]")
-    if residual is not None and (residual.shape != (T, n_out) or (w.is_cuda and (residual.stride(1) != 1 or residual.dtype not in (torch.bfloat16, torch.float32)))):
+    if residual is not None and (residual.shape != (T, n_out) or (cuda and (residual.stride(1) != 1 or residual.dtype not in (torch.bfloat16, torch.float32)))):
         raise ValueError(f"the residual rows are [{T}, {n_out}] in bfloat16 or float32")
-    if out is not None and (out.shape != (T, n_out) or out.stride(1) != 1 or (w.is_cuda and out.dtype != (torch.float32 if out_fp32 else torch.bfloat16))):
+    if out is not None and (out.shape != (T, n_out) or out.stride(1) != 1 or (cuda and out.dtype != (torch.float32 if out_fp32 else torch.bfloat16))):
         raise ValueError(f"the output is [{T}, {n_out}] in {'float32' if out_fp32 else 'bfloat16'}")
-    if not w.is_cuda:
+    if not cuda:
         xv = x.dequantize() if given else fp4_matrix.quantize(x, w.form).dequantize()
         if pair:
             y = ref.gate_up_act(xv, w.dequantize(), bias, "silu", True)
@@ -497,19 +500,17 @@ def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=N
         y = y.to(torch.float32 if out_fp32 else torch.bfloat16 if given else x.dtype)
         return y if out is None else out.copy_(y)
     if out is None:
-        out = torch.empty(T, n_out, dtype=torch.float32 if out_fp32 else torch.bfloat16, device=w.device)
-    form, ws = fp4_matrix.FORMS[w.form], workspace(w.device)
+        out = torch.empty(T, n_out, dtype=torch.float32 if out_fp32 else torch.bfloat16, device=dev)
     if given:
-        rows, ldx, x32, a = None, 0, 0, x.data
+        rows, ldx, x32, a = None, 0, False, x.data
     else:
         if x.stride(1) != 1:
             x = x.contiguous()
-        rows, ldx, x32 = x.data_ptr(), x.stride(0), int(x.dtype == torch.float32)
-        a = torch.empty(fp4_matrix.matrix_bytes(T, K, w.form), dtype=torch.uint8, device=w.device)
-    with _on(w.device):
-        _lib.check(_lib.lib().ogb_linear_fp4(rows, ldx, x32, a.data_ptr(), T, w.data.data_ptr(), N, K, form, out.data_ptr(), out.stride(0), int(out_fp32), int(pair),
-                                             _ptr(bias), _ptr(residual), residual.stride(0) if residual is not None else 0,
-                                             int(residual is not None and residual.dtype == torch.float32), ws.status, ws.sm_count, _stream()), "linear_fp4")
+        rows, ldx, x32 = x.data_ptr(), x.stride(0), x.dtype == torch.float32
+        a = torch.empty(fp4_matrix.matrix_bytes(T, K, w.form), dtype=torch.uint8, device=dev)
+    ws = workspace(dev)
+    _call_on(ws.index, "ogb_linear_fp4", rows, ldx, x32, a.data_ptr(), T, data.data_ptr(), N, K, fp4_matrix.FORMS[w.form], out.data_ptr(), out.stride(0), out_fp32, pair,
+             _ptr(bias), _ptr(residual), 0 if residual is None else residual.stride(0), residual is not None and residual.dtype == torch.float32, ws.status, ws.sm_count)
     return out
 
 
@@ -1004,15 +1005,13 @@ def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, 
         return ref.moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, top, weights, act, alpha, limit)
     if x.dtype != torch.bfloat16 or any(t.dtype != torch.bfloat16 or not t.is_contiguous() for t in tensors):
         raise ValueError("moe_few_tokens takes contiguous bfloat16 weights and biases, and bfloat16 rows")
-    if x.stride(1) != 1:
-        x = x.contiguous()
+    if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
     out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
     scratch = torch.empty(_lib.lib().ogb_moe_few_scratch_bytes(T, top, I), dtype=torch.uint8, device=x.device)
-    with _on(x.device):
-        _lib.check(_lib.lib().ogb_moe_few_tokens(x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),
-                                                 _ptr(gate_up_b), (down_w.packed if packed else down_w).data_ptr(), _ptr(down_b), out.data_ptr(), T, H, I, E, top,
-                                                 _FEW_RULES[weights], (1 if gate_up_w.half else 2) if packed else 0, _FEW_ACTS[act], float(alpha), float(limit),
-                                                 scratch.data_ptr(), _stream()), "moe_few_tokens")
+    _call_on(x.get_device(), "ogb_moe_few_tokens", x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),
+             _ptr(gate_up_b), (down_w.packed if packed else down_w).data_ptr(), _ptr(down_b), out.data_ptr(), T, H, I, E, top, _FEW_RULES[weights],
+             (1 if gate_up_w.half else 2) if packed else 0, _FEW_ACTS[act], alpha, limit, scratch.data_ptr())
     return out
 
 
