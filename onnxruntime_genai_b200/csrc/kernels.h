@@ -354,7 +354,7 @@ int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T
 long long ogb_moe_few_scratch_bytes(int T, int top, int I);     // -1: refused
 int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b, const void* down,
                        const void* down_b, void* out, int T, int H, int I, int E, int top, int rule, int weights, int act, float alpha, float limit,
-                       void* scratch, void* stream);
+                       void* scratch, int* status, int sm_count, void* stream);
 
 // ---- sampling.cu
 int ogb_sample(const float* logits, long long row_stride, int rows, int vocab, const int32_t* top_k, const float* top_p,

@@ -25,11 +25,12 @@ namespace ogb {
 enum FewWeights : int { FEW_BF16 = 0, FEW_FP4_F16 = 1, FEW_FP4_BF16 = 2 };   // packed: the records of gemm_fp4.cu in their two forms
 constexpr int FEW_TOKENS = 8, FEW_TOP = 32, FEW_EXPERTS = 1024, FEW_MET = FEW_TOKENS * FEW_TOP;
 constexpr int FEW_CLUSTER = 8;
-constexpr int FEW_A_THREADS = 256, FEW_B_THREADS = 512;
-constexpr size_t FEW_SMEM_TWO = 112 * 1024;
+constexpr int FEW_THREADS = 288, FEW_STAGES = 16;
+constexpr size_t FEW_SMEM_TWO = 112 * 1024, FEW_SMEM_ONE = 227 * 1024;          // shared memory of a CTA, with two or one on an SM
+constexpr int FEW_DOWN_RING = 72 * 1024;
 
 // What the first kernel leaves for the second.
-struct FewPlan {
+struct alignas(16) FewPlan {
   int met, unused[3];                       // experts that any token meets, in ascending order
   int expert[FEW_MET];
   uint8_t slot[FEW_MET][FEW_TOKENS];        // which choice of the token the expert is; 255: none
@@ -52,6 +53,8 @@ struct FewArgs {
   float alpha, limit;
   FewPlan* plan;
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
+  int stages, splits;   // of the first kernel's ring; CTAs of a cluster of the second
+  int* status;
 };
 
 // ------------------------------------------------------------------------------- operands
@@ -68,114 +71,55 @@ __device__ __forceinline__ void mma_bf16_32(float (&d)[4], const uint4& r0, cons
   mma_bf16_16816(d, r0.x, r1.x, r0.y, r1.y, b.x, b.y);
   mma_bf16_16816(d, r0.z, r1.z, r0.w, r1.w, b.z, b.w);
 }
-__device__ __forceinline__ uint4 ld_stream(const void* p) {         // weights are read once: they need no place in L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ld_stream2(const void* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
-// Two weight rows of a warp's tile (row lane / 4 of each half), k values 64 c .. 64 c + 63: a lane's 16 of each row.
-template <int W> struct FewChunk;
-template <> struct FewChunk<FEW_BF16> {
-  uint4 a[2][2];
-  // p0, p1: the lane's place in the rows; left: k values from there to the rows' end
-  __device__ __forceinline__ void load(const uint8_t* p0, const uint8_t* p1, int left) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    a[0][0] = left > 0 ? ld_stream(p0) : zero;
-    a[1][0] = left > 0 ? ld_stream(p1) : zero;
-    a[0][1] = left > 32 ? ld_stream(p0 + 64) : zero;
-    a[1][1] = left > 32 ? ld_stream(p1 + 64) : zero;
-  }
-  __device__ __forceinline__ void mma(float (&acc)[4], const uint4 (&b)[2]) const {
-    mma_bf16_32(acc, a[0][0], a[1][0], b[0]);
-    mma_bf16_32(acc, a[0][1], a[1][1], b[1]);
-  }
-};
-__device__ __forceinline__ float fp4_half_scale(uint32_t s) { return __uint_as_float((s - 6u) << 23); }      // the records hold code + 6
-template <> struct FewChunk<FEW_FP4_F16> {
-  uint2 q[2];
-  uint16_t s[2];
-  // p: the lane's eight bytes of a row's record, ps: the row's two scales
-  __device__ __forceinline__ void load(const uint8_t* p0, const uint8_t* p1, const uint8_t* ps0, const uint8_t* ps1) {
-    q[0] = ld_stream2(p0);
-    q[1] = ld_stream2(p1);
-    s[0] = __ldg(reinterpret_cast<const uint16_t*>(ps0));
-    s[1] = __ldg(reinterpret_cast<const uint16_t*>(ps1));
-  }
-  // a block of 32 has one scale per row: its sum is scaled as a whole
-  __device__ __forceinline__ void mma(float (&acc)[4], const uint4 (&b)[2]) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t u[4], v[4];
-      cvt_e2m1x8_f16(i ? q[0].y : q[0].x, u);
-      cvt_e2m1x8_f16(i ? q[1].y : q[1].x, v);
-      float t[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_f16_16816(t, u[0], v[0], u[1], v[1], b[i].x, b[i].y);
-      mma_f16_16816(t, u[2], v[2], u[3], v[3], b[i].z, b[i].w);
-      const float s0 = fp4_half_scale(i ? s[0] >> 8 : s[0] & 255), s1 = fp4_half_scale(i ? s[1] >> 8 : s[1] & 255);
-      acc[0] = fmaf(t[0], s0, acc[0]);
-      acc[1] = fmaf(t[1], s0, acc[1]);
-      acc[2] = fmaf(t[2], s1, acc[2]);
-      acc[3] = fmaf(t[3], s1, acc[3]);
-    }
-  }
-};
-template <> struct FewChunk<FEW_FP4_BF16> {
-  uint32_t q[2][2];
-  uint16_t s[2];
-  __device__ __forceinline__ void load(const uint8_t* p0, const uint8_t* p1, const uint8_t* ps0, const uint8_t* ps1) {
-    q[0][0] = __ldg(reinterpret_cast<const uint32_t*>(p0));
-    q[0][1] = __ldg(reinterpret_cast<const uint32_t*>(p0 + 16));
-    q[1][0] = __ldg(reinterpret_cast<const uint32_t*>(p1));
-    q[1][1] = __ldg(reinterpret_cast<const uint32_t*>(p1 + 16));
-    s[0] = __ldg(reinterpret_cast<const uint16_t*>(ps0));
-    s[1] = __ldg(reinterpret_cast<const uint16_t*>(ps1));
-  }
-  __device__ __forceinline__ void mma(float (&acc)[4], const uint4 (&b)[2]) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      mma_bf16_32(acc, deq_fp4_word_bf16(q[0][i], i ? s[0] >> 8 : s[0] & 255), deq_fp4_word_bf16(q[1][i], i ? s[1] >> 8 : s[1] & 255), b[i]);
-  }
-};
-
-// A place in the weights: the rows r0 and r1 (in one tile of 128) of expert e, going up in steps of 64 k values.
+// A stage of the ring holds CHUNKS steps of 64 k values of a tile of 128 weight rows, as they lie in memory: packed records, or (bf16) a box of 64 columns with
+// the 128-byte swizzle.  A warp multiplies 16 of the rows, r0 = the row of lanes 4 g .. 4 g + 3 in the tile's first half of its 16, r1 in the second.
 template <int W>
-struct FewRows {
-  const uint8_t *p0, *p1, *s0, *s1;
-  long long step;
-  int left;
-  __device__ __forceinline__ void seek(const void* w, int e, int N, int K, int r0, int r1, int chunk, int q) {
-    const uint8_t* base = static_cast<const uint8_t*>(w);
+struct FewTile {
+  static constexpr int CHUNKS = W == FEW_BF16 ? 1 : 2;
+  static constexpr int BYTES = W == FEW_BF16 ? 128 * 128 : FP4_RECORD_BYTES;       // of a step
+  static __device__ __forceinline__ void mma(float (&acc)[4], const uint8_t* tile, int r0, int r1, int g, int q, const uint4 (&b)[2]) {
     if constexpr (W == FEW_BF16) {
-      left = K - chunk * 64 - q * 8;
-      p0 = base + (((long long)e * N + r0) * K + chunk * 64 + q * 8) * 2;
-      p1 = base + (((long long)e * N + r1) * K + chunk * 64 + q * 8) * 2;
-      step = 128;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = ((q + 4 * i) ^ g) << 4;
+        mma_bf16_32(acc, *reinterpret_cast<const uint4*>(tile + r0 * 128 + c), *reinterpret_cast<const uint4*>(tile + r1 * 128 + c), b[i]);
+      }
+    } else if constexpr (W == FEW_FP4_F16) {
+      const uint2 q0 = *reinterpret_cast<const uint2*>(tile + r0 * 32 + q * 8), q1 = *reinterpret_cast<const uint2*>(tile + r1 * 32 + q * 8);
+      const uint32_t s0 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r0 * 2), s1 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r1 * 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {                       // a block of 32 has one scale per row (the records hold code + 6): its sum is scaled as a whole
+        uint32_t u[4], v[4];
+        cvt_e2m1x8_f16(i ? q0.y : q0.x, u);
+        cvt_e2m1x8_f16(i ? q1.y : q1.x, v);
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16_16816(t, u[0], v[0], u[1], v[1], b[i].x, b[i].y);
+        mma_f16_16816(t, u[2], v[2], u[3], v[3], b[i].z, b[i].w);
+        const float f0 = __uint_as_float(((i ? s0 >> 8 : s0 & 255u) - 6u) << 23), f1 = __uint_as_float(((i ? s1 >> 8 : s1 & 255u) - 6u) << 23);
+        acc[0] = fmaf(t[0], f0, acc[0]);
+        acc[1] = fmaf(t[1], f0, acc[1]);
+        acc[2] = fmaf(t[2], f1, acc[2]);
+        acc[3] = fmaf(t[3], f1, acc[3]);
+      }
     } else {
-      const int tiles = (N + 127) >> 7;
-      const uint8_t* rec = base + (((long long)e * (K >> 6) + chunk) * tiles + (r0 >> 7)) * FP4_RECORD_BYTES;
-      const int at = W == FEW_FP4_F16 ? q * 8 : q * 4;
-      p0 = rec + (r0 & 127) * 32 + at;
-      p1 = rec + (r1 & 127) * 32 + at;
-      s0 = rec + 128 * 32 + (r0 & 127) * 2;
-      s1 = rec + 128 * 32 + (r1 & 127) * 2;
-      step = (long long)tiles * FP4_RECORD_BYTES;
+      const uint32_t s0 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r0 * 2), s1 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r1 * 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        mma_bf16_32(acc, deq_fp4_word_bf16(*reinterpret_cast<const uint32_t*>(tile + r0 * 32 + i * 16 + q * 4), i ? s0 >> 8 : s0 & 255u),
+                    deq_fp4_word_bf16(*reinterpret_cast<const uint32_t*>(tile + r1 * 32 + i * 16 + q * 4), i ? s1 >> 8 : s1 & 255u), b[i]);
     }
   }
-  __device__ __forceinline__ void load(FewChunk<W>& c) const {
-    if constexpr (W == FEW_BF16) c.load(p0, p1, left); else c.load(p0, p1, s0, s1);
-  }
-  __device__ __forceinline__ void next() {
-    p0 += step;
-    p1 += step;
-    if constexpr (W == FEW_BF16) left -= 64; else { s0 += step; s1 += step; }
-  }
 };
+// Copies step `chunk` of 128 weight rows (tile `tile` of expert e's rows) to shared memory; by one thread.
+template <int W>
+__device__ __forceinline__ void few_copy(uint8_t* dst, uint64_t* bar, const CUtensorMap* map, const void* packed, int e, int tile, int chunk, int N, int K) {
+  if constexpr (W == FEW_BF16) {
+    tma_load_2d(dst, map, bar, chunk * 64, e * N + tile * 128);
+  } else {
+    const int tiles = (N + 127) >> 7;
+    bulk_copy_g2s(dst, static_cast<const uint8_t*>(packed) + (((long long)e * (K >> 6) + chunk) * tiles + tile) * FP4_RECORD_BYTES, FP4_RECORD_BYTES, bar);
+  }
+}
 
 // Eight 16-bit values in the order in which a lane's eight weights of a row come out of their load: pairs (0, 1) (2, 3) .. or, from records in fp16 form,
 // (0, 4) (1, 5) (2, 6) (3, 7).
@@ -186,14 +130,50 @@ __device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // 
   return r;
 }
 
+// ------------------------------------------------------------------------------- ring of copies
+// Warp 8 copies, warps 0 .. 7 multiply.  All waits are bounded; after a failed one every warp leaves its loop.
+struct FewBars { uint64_t full[FEW_STAGES], empty[FEW_STAGES]; int abort; };
+__device__ __forceinline__ void few_init(FewBars& b, int stages) {
+  for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], 1); mbar_init(&b.empty[s], 8); }
+  b.abort = 0;
+  mbar_fence_init();
+}
+struct FewRing {
+  int stages, s = 0, filled = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    ++filled;
+    if (++s == stages) { s = 0; ph ^= 1; }
+  }
+  __device__ __forceinline__ bool fail(FewBars& b, int* status) { atomicMax(status, OGB_ERR_WAIT_TMA); *reinterpret_cast<volatile int*>(&b.abort) = 1; return false; }
+  __device__ __forceinline__ bool wait_empty(FewBars& b, int* status) {
+    if (filled < stages) return true;
+    return __all_sync(0xffffffffu, mbar_wait_bounded(&b.empty[s], ph ^ 1, &b.abort)) || fail(b, status);
+  }
+  // A consumer warp hands the stage before this one back only here.  Directly behind the products of its own stage the arrival could overtake reads of shared
+  // memory that are still on their way (the compiler may put it in front of the products that wait for them; seen as single wrong rows); behind the wait for the
+  // next stage all products, and so all reads, have been issued and answered.
+  __device__ __forceinline__ bool wait_full(FewBars& b, int* status, int lane) {
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&b.full[s], ph, &b.abort))) return fail(b, status);
+    if (filled > 0 && lane == 0) mbar_arrive(&b.empty[(s == 0 ? stages : s) - 1]);
+    return true;
+  }
+  __device__ __forceinline__ void drain(FewBars& b) {          // copies in flight still write shared memory: give them time to land
+    volatile int never = 0;
+    for (int i = max(0, filled - stages); i < filled; ++i) mbar_wait_bounded(&b.full[i % stages], (i / stages) & 1, &never, 200000000ull);
+  }
+};
+
 // ------------------------------------------------------------------------------- router, choice
 // Shared memory of the first kernel.
 struct FewShared {
-  float red[8][16 * FEW_TOKENS];
+  FewBars bars;
+  float red[FEW_THREADS / 32][16 * FEW_TOKENS];
   uint32_t top[FEW_TOKENS];          // bits of the rows' largest magnitudes
   uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
   FewPlan plan;
 };
+static_assert(sizeof(FewShared) % 16 == 0, "16-byte accesses to what follows");
 
 // Power of two that brings a row's largest magnitude (its bits) to 2^14 .. 2^15
 __device__ __forceinline__ int few_shift(uint32_t top) { return top >= 0x7f800000u ? 0 : min(14 - (int(top >> 23) - 127), 126); }
@@ -240,18 +220,21 @@ __device__ __forceinline__ void few_choose(const float* row, int E, int top, int
 }
 
 template <int W>
-__global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const FewArgs p) {
-  constexpr int DEPTH = W == FEW_BF16 ? 4 : 8;
-  extern __shared__ __align__(16) uint8_t smem[];
-  FewShared& sh = *reinterpret_cast<FewShared*>(smem);
-  float* logits = reinterpret_cast<float*>(smem + sizeof(FewShared));                       // [T][E]
+__global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
+  using Tile = FewTile<W>;
+  constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  FewShared& sh = *reinterpret_cast<FewShared*>(ring + p.stages * STAGE);
+  float* logits = reinterpret_cast<float*>(&sh + 1);                                         // [T][E]
   const int Hp = (p.H + 63) / 64 * 64, xs_ld = Hp + 32;              // 16-bit values a row: neighbours start 64 bytes apart in the banks
-  uint16_t* xs = reinterpret_cast<uint16_t*>(smem + sizeof(FewShared) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16);
+  uint16_t* xs = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(logits) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = int(cluster_ctarank());
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the others' shared memory is written only once they run
-  for (int e = threadIdx.x; e < p.E; e += FEW_A_THREADS) sh.mask[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) sh.mask[e] = 0;
   if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
+  if (threadIdx.x == 0) few_init(sh.bars, p.stages);
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
@@ -260,7 +243,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
   const int parts = (Hp + 255) >> 8, pieces = p.T * parts;
   if (W == FEW_FP4_F16) {
 #pragma unroll 4
-    for (int i = warp; i < pieces; i += 8) {
+    for (int i = warp; i < pieces; i += FEW_THREADS / 32) {
       const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
       const uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -282,7 +265,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
     const __nv_bfloat16* w0 = p.router + (long long)(r0 ? e0 + g : 0) * p.H;
     const __nv_bfloat16* w1 = p.router + (long long)(r1 ? e0 + g + 8 : 0) * p.H;
 #pragma unroll 4
-    for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += 256) {
+    for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += FEW_THREADS) {
       const bool in = k < p.H;
       const uint4 a0 = r0 && in ? *reinterpret_cast<const uint4*>(w0 + k) : zero, a1 = r1 && in ? *reinterpret_cast<const uint4*>(w1 + k) : zero;
       const uint4 b = g < p.T && in ? *reinterpret_cast<const uint4*>(p.x + g * p.ldx + k) : zero;
@@ -297,7 +280,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
       if (e < e_end && t < p.T) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) v += sh.red[w][threadIdx.x];
+        for (int w = 0; w < FEW_THREADS / 32; ++w) v += sh.red[w][threadIdx.x];
         if (p.router_b) v += bf2f(p.router_b[e]);
         const uint32_t at = smem_u32(logits + t * p.E + e);
 #pragma unroll
@@ -309,7 +292,7 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   // the rows as the products read them
 #pragma unroll 4
-  for (int i = warp; i < pieces; i += 8) {
+  for (int i = warp; i < pieces; i += FEW_THREADS / 32) {
     const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
     uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
     if (W == FEW_FP4_F16) {
@@ -354,124 +337,144 @@ __global__ void __launch_bounds__(FEW_A_THREADS, 2) few_gate_up_kernel(const Few
   __syncthreads();
   if (blockIdx.x == 0) {
     const uint4* src = reinterpret_cast<const uint4*>(&sh.plan);
-    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_A_THREADS) reinterpret_cast<uint4*>(p.plan)[i] = src[i];
+    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_THREADS) reinterpret_cast<uint4*>(p.plan)[i] = src[i];
   }
 
-  // gate and up rows: a unit is eight features of a met expert; neighbours in memory are at work at the same time
-  const int blocks = p.I >> 3, units = sh.plan.met * blocks, stride = int(gridDim.x) * 8, chunks = Hp >> 6;
-  FewChunk<W> ring[DEPTH];
-  FewRows<W> rows;
-  int lu = int(blockIdx.x) + int(gridDim.x) * warp, lc = 0;                  // where the loads are
-  auto seek = [&]() {
-    if (lu < units) {
-      const int d = lu / blocks, f = (lu - d * blocks) * 8 + g, r = (f >> 6) * 128 + (f & 63);
-      rows.seek(p.gate_up, sh.plan.expert[d], 2 * p.I, p.H, r, r + 64, 0, q);
-    }
-  };
-  auto fetch = [&](FewChunk<W>& c) {
-    if (lu >= units) return;
-    rows.load(c);
-    if (++lc < chunks) { rows.next(); return; }
-    lc = 0;
-    lu += stride;
-    seek();
-  };
-  seek();
-#pragma unroll
-  for (int i = 0; i < DEPTH; ++i) fetch(ring[i]);
-  const uint16_t* xt = xs + (g < p.T ? g : 0) * xs_ld + q * 8;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  int u = int(blockIdx.x) + int(gridDim.x) * warp, c = 0;                    // where the products are
-  while (u < units) {
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (u >= units) break;
-      // columns beyond the tokens: any numbers, they are not looked at
-      const uint4 b[2] = {*reinterpret_cast<const uint4*>(xt + c * 64), *reinterpret_cast<const uint4*>(xt + c * 64 + 32)};
-      ring[i].mma(acc, b);
-      fetch(ring[i]);
-      if (++c < chunks) continue;
-      const int d = u / blocks, i0 = (u - d * blocks) * 8, e = sh.plan.expert[d], r = ((i0 + g) >> 6) * 128 + ((i0 + g) & 63);
-      const float bg = p.gate_up_b ? bf2f(p.gate_up_b[(long long)e * 2 * p.I + r]) : 0.f, bu = p.gate_up_b ? bf2f(p.gate_up_b[(long long)e * 2 * p.I + r + 64]) : 0.f;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int t = q * 2 + j, slot = sh.plan.slot[d][t];
-        if (slot != 255) {
-          const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) : 1.f;
-          float gate = fmaf(acc[j], s, bg), up = fmaf(acc[2 + j], s, bu), v;
-          if (p.act == 2) {
-            if (p.limit > 0.f) {             // (comparisons, not minima: what is not a number stays that)
-              gate = gate > p.limit ? p.limit : gate;
-              up = up > p.limit ? p.limit : up < -p.limit ? -p.limit : up;
-            }
-            v = gate / (1.f + expf(-p.alpha * gate)) * (up + 1.f);
-          } else {
-            v = gate / (1.f + expf(-gate)) * up;
-          }
-          const int pair = t * p.top + slot;
-          v *= sh.plan.share[pair];
-          const uint32_t bits = W == FEW_FP4_F16 ? f16x2_sat(v, 0.f) : pack_bf16x2(v, 0.f);
-          p.h[(long long)pair * p.I + i0 + few_place<W>(g)] = uint16_t(bits);
+  // gate and up rows: an item is 64 features of a met expert, 128 rows that lie together; a warp takes eight features
+  const int tiles = p.I >> 6, items = sh.plan.met * tiles, chunks = Hp >> 6;
+  if (warp == 8) {
+    FewRing r{p.stages};
+    bool ok = true;
+    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
+      const int e = sh.plan.expert[item / tiles], tile = item % tiles;
+      for (int c = 0; c < chunks; c += Tile::CHUNKS) {
+        ok = r.wait_empty(sh.bars, p.status);
+        if (!ok) break;
+        if (elect_one()) {
+          const int n = min(Tile::CHUNKS, chunks - c);
+          uint64_t* bar = &sh.bars.full[r.s];
+          mbar_expect_tx(bar, n * Tile::BYTES);
+          for (int i = 0; i < n; ++i) few_copy<W>(ring + r.s * STAGE + i * Tile::BYTES, bar, &map, p.gate_up, e, tile, c + i, 2 * p.I, p.H);
         }
-        acc[j] = acc[2 + j] = 0.f;
+        __syncwarp();
+        r.next();
       }
-      c = 0;
-      u += stride;
+    }
+    if (!ok) r.drain(sh.bars);
+    return;
+  }
+  FewRing r{p.stages};
+  const uint16_t* xt = xs + (g < p.T ? g : 0) * xs_ld + q * 8;           // (columns beyond the tokens: any numbers, they are not looked at)
+  const int r0 = warp * 8 + g;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int d = item / tiles, tile = item - d * tiles, e = sh.plan.expert[d], i0 = tile * 64 + warp * 8;
+    const long long row = (long long)e * 2 * p.I + tile * 128 + r0;
+    const float bg = p.gate_up_b ? bf2f(p.gate_up_b[row]) : 0.f, bu = p.gate_up_b ? bf2f(p.gate_up_b[row + 64]) : 0.f;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < chunks; c += Tile::CHUNKS) {
+      if (!r.wait_full(sh.bars, p.status, lane)) return;
+#pragma unroll
+      for (int i = 0; i < Tile::CHUNKS; ++i) {
+        if (i > 0 && c + i >= chunks) break;
+        const uint4 b[2] = {*reinterpret_cast<const uint4*>(xt + (c + i) * 64), *reinterpret_cast<const uint4*>(xt + (c + i) * 64 + 32)};
+        Tile::mma(acc, ring + r.s * STAGE + i * Tile::BYTES, r0, r0 + 64, g, q, b);
+      }
+      r.next();
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int t = q * 2 + j, slot = sh.plan.slot[d][t];
+      if (slot == 255) continue;
+      const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) : 1.f;
+      float gate = fmaf(acc[j], s, bg), up = fmaf(acc[2 + j], s, bu), v = gate;
+      if (p.act == 2) {
+        if (p.limit > 0.f) {             // (comparisons, not minima: what is not a number stays that)
+          gate = gate > p.limit ? p.limit : gate;
+          up = up > p.limit ? p.limit : up < -p.limit ? -p.limit : up;
+        }
+        v = p.alpha * gate;
+        up += 1.f;
+      }
+      const int pair = t * p.top + slot;
+      v = gate / (1.f + expf(-v)) * up * sh.plan.share[pair];
+      p.h[(long long)pair * p.I + i0 + few_place<W>(g)] = uint16_t(W == FEW_FP4_F16 ? f16x2_sat(v, 0.f) : pack_bf16x2(v, 0.f));
     }
   }
 }
 
+// A cluster computes 128 columns of the output, its CTAs take equal parts of the sequence (expert, k); partial sums are sent to the CTA that finishes their rows.
 template <int W>
-__global__ void __launch_bounds__(FEW_B_THREADS, 1) few_down_kernel(const FewArgs p) {
-  constexpr int DEPTH = W == FEW_BF16 ? 3 : 6, WARPS = FEW_B_THREADS / 32;
-  __shared__ FewPlan plan;
-  __shared__ float red[WARPS][16 * FEW_TOKENS];
+__global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
+  using Tile = FewTile<W>;
+  constexpr int H_LD = Tile::CHUNKS * 128 + 64, H_OFF = Tile::CHUNKS * Tile::BYTES, STAGE = (H_OFF + FEW_TOKENS * H_LD + 1023) / 1024 * 1024;
+  constexpr int STAGES = FEW_DOWN_RING / STAGE < FEW_STAGES ? FEW_DOWN_RING / STAGE : FEW_STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ FewBars bars;
+  __shared__ __align__(16) FewPlan plan;
+  __shared__ __align__(16) float red[128 * FEW_TOKENS];                         // [sender][rows of this CTA: 128 / splits][token]
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int n0 = blockIdx.x * 16;
+  const int rank = int(cluster_ctarank()), splits = p.splits, tile = blockIdx.x / splits;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  if (threadIdx.x == 0) few_init(bars, STAGES);
   pdl_wait();
   pdl_launch_dependents();
   {
     const uint4* src = reinterpret_cast<const uint4*>(p.plan);
-    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_B_THREADS) reinterpret_cast<uint4*>(&plan)[i] = src[i];
+    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_THREADS) reinterpret_cast<uint4*>(&plan)[i] = src[i];
   }
   __syncthreads();
-  const int chunks = p.I >> 6, total = plan.met * chunks;
-  const int lo = int((long long)total * warp / WARPS), hi = int((long long)total * (warp + 1) / WARPS);
-  const int r0 = min(n0 + g, p.H - 1), r1 = min(n0 + g + 8, p.H - 1);        // rows past the end: any, they are not stored
-
-  struct Item { FewChunk<W> w; uint4 h[2]; };
-  Item ring[DEPTH];
-  FewRows<W> rows;
-  const uint16_t* hp = nullptr;                                               // this lane's token's activations of the expert; null: it does not meet it
-  int at = lo, ld = 0, lc = 0;
-  auto seek = [&]() {
-    if (at >= hi) return;
-    ld = at / chunks;
-    lc = at - ld * chunks;
-    rows.seek(p.down, plan.expert[ld], p.H, p.I, r0, r1, lc, q);
-    const int slot = plan.slot[ld][g];
-    hp = slot == 255 ? nullptr : p.h + (long long)(g * p.top + slot) * p.I + lc * 64 + q * 8;
-  };
-  auto fetch = [&](Item& it) {
-    if (at >= hi) return;
-    rows.load(it.w);
-    it.h[0] = hp ? *reinterpret_cast<const uint4*>(hp) : make_uint4(0, 0, 0, 0);
-    it.h[1] = hp ? *reinterpret_cast<const uint4*>(hp + 32) : make_uint4(0, 0, 0, 0);
-    ++at;
-    if (++lc < chunks) { rows.next(); if (hp) hp += 64; } else seek();
-  };
-  seek();
+  const int chunks = p.I >> 6, steps = (chunks + Tile::CHUNKS - 1) / Tile::CHUNKS, total = plan.met * steps;
+  const int lo = int((long long)total * rank / splits), hi = int((long long)total * (rank + 1) / splits);
+  bool ok = true;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (warp == 8) {
+    FewRing r{STAGES};
+    int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
+    for (int i = lo; i < hi; ++i) {
+      ok = r.wait_empty(bars, p.status);
+      if (!ok) break;
+      if (elect_one()) {
+        const int n = min(Tile::CHUNKS, chunks - c), e = plan.expert[d];
+        const uint2 sl = *reinterpret_cast<const uint2*>(plan.slot[d]);
+        uint8_t* st = ring + r.s * STAGE;
+        uint64_t* bar = &bars.full[r.s];
+        int meet = 0;
+        for (int t = 0; t < p.T; ++t) meet += ((t < 4 ? sl.x : sl.y) >> (t & 3) * 8 & 255u) != 255u;
+        mbar_expect_tx(bar, n * (Tile::BYTES + meet * 128));
+        for (int j = 0; j < n; ++j) few_copy<W>(st + j * Tile::BYTES, bar, &map, p.down, e, tile, c + j, p.H, p.I);
+        for (int t = 0; t < p.T; ++t) {
+          const uint32_t slot = (t < 4 ? sl.x : sl.y) >> (t & 3) * 8 & 255u;
+          if (slot != 255u) bulk_copy_g2s(st + H_OFF + t * H_LD, p.h + (long long)(t * p.top + slot) * p.I + c * 64, n * 128, bar);
+        }
+      }
+      __syncwarp();
+      r.next();
+      c += Tile::CHUNKS;
+      if (c >= chunks) { c = 0; ++d; }
+    }
+    if (!ok) r.drain(bars);
+  } else {
+    FewRing r{STAGES};
+    int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const int r0 = warp * 16 + g;
+    for (int i = lo; i < hi; ++i) {
+      ok = r.wait_full(bars, p.status, lane);
+      if (!ok) break;
+      const uint8_t* st = ring + r.s * STAGE;
+      const bool mine = plan.slot[d][g] != 255;
 #pragma unroll
-  for (int i = 0; i < DEPTH; ++i) fetch(ring[i]);
-  float sum[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  int c = lo < hi ? lo % chunks : 0, d = lo < hi ? lo / chunks : 0;
-  for (int i0 = lo; i0 < hi; i0 += DEPTH) {
-#pragma unroll
-    for (int i = 0; i < DEPTH; ++i) {
-      if (i0 + i >= hi) break;
-      ring[i].w.mma(acc, ring[i].h);
-      fetch(ring[i]);
-      if (++c < chunks && i0 + i + 1 < hi) continue;
+      for (int j = 0; j < Tile::CHUNKS; ++j) {
+        if (j > 0 && c + j >= chunks) break;
+        const uint8_t* hs = st + H_OFF + g * H_LD + j * 128 + q * 16;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        const uint4 b[2] = {mine ? *reinterpret_cast<const uint4*>(hs) : zero, mine ? *reinterpret_cast<const uint4*>(hs + 64) : zero};
+        Tile::mma(acc, st + j * Tile::BYTES, r0, r0 + 8, g, q, b);
+      }
+      r.next();
+      c += Tile::CHUNKS;
+      if (c < chunks && i + 1 < hi) continue;
       // an expert's part is done: it counts for the tokens that meet it (weights that are not numbers stay with them)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -482,29 +485,47 @@ __global__ void __launch_bounds__(FEW_B_THREADS, 1) few_down_kernel(const FewArg
       ++d;
     }
   }
-  *reinterpret_cast<float2*>(&red[warp][g * 8 + q * 2]) = make_float2(sum[0], sum[1]);
-  *reinterpret_cast<float2*>(&red[warp][(g + 8) * 8 + q * 2]) = make_float2(sum[2], sum[3]);
-  __syncthreads();
-  if (threadIdx.x < 128) {
-    const int n = n0 + int(threadIdx.x & 15), t = threadIdx.x >> 4;
-    if (t < p.T && n < p.H) {
-      float v = 0.f;
+  // rows of the tile are dealt out to the cluster's CTAs, a multiple of 16 each
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // of the arrival at the start
+  const int rows = 128 / splits;
+  if (warp < 8) {
+    const int owner = warp * 16 / rows, l = warp * 16 - owner * rows;
+    const uint32_t at = dsmem_addr(smem_u32(&red[(rank * rows + l + g) * FEW_TOKENS + q * 2]), uint32_t(owner));
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) v += red[w][(threadIdx.x & 15) * 8 + t];
-      if (p.down_b)
-        for (int j = 0; j < p.top; ++j) v += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
-      p.out[(long long)t * p.H + n] = f2bf(v);
-    }
+    for (int j = 0; j < 2; ++j)
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at + j * 8 * FEW_TOKENS * 4), "f"(sum[j * 2]), "f"(sum[j * 2 + 1]) : "memory");
+  }
+  cluster_sync_all();
+  for (int i = threadIdx.x; i < rows * FEW_TOKENS; i += FEW_THREADS) {
+    const int t = i / rows, l = i - t * rows, n = tile * 128 + rank * rows + l;
+    if (t >= p.T || n >= p.H) continue;
+    float v = 0.f;
+    for (int s = 0; s < splits; ++s) v += red[(s * rows + l) * FEW_TOKENS + t];
+    if (p.down_b)
+      for (int j = 0; j < p.top; ++j) v += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
+    p.out[(long long)t * p.H + n] = f2bf(v);
   }
 }
 
+// --------------------------------------------------------------------------------- host side
+bool MakeMapBf16(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows);  // gemm_tcgen05.cu
+
 template <int W>
-static int LaunchFew(const FewArgs& p, cudaStream_t stream) {
-  const int Hp = (p.H + 63) / 64 * 64, xs_ld = Hp + 32;
-  const size_t smem = sizeof(FewShared) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16 + size_t(p.T) * xs_ld * 2;
-  if (smem > 227 * 1024) return -5;
-  static bool configured[OGB_MAX_DEVICES] = {};
-  if (!set_max_dyn_smem(few_gate_up_kernel<W>, 227 * 1024, configured)) return -3;
+static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
+  using Tile = FewTile<W>;
+  constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
+  const int Hp = (p.H + 63) / 64 * 64;
+  const size_t fixed = 1024 + sizeof(FewShared) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16 + size_t(p.T) * (Hp + 32) * 2;
+  // Two CTAs an SM where that leaves each a ring of 48 KiB: more warps to expand and multiply; else one with what there is.
+  const int two = fixed + 48 * 1024 <= FEW_SMEM_TWO;
+  const size_t room = two ? FEW_SMEM_TWO : FEW_SMEM_ONE;
+  if (fixed + 2 * STAGE > room) return -5;
+  p.stages = int(min(size_t(FEW_STAGES), (room - fixed) / STAGE));
+  CUtensorMap gate_up = {}, down = {};
+  if (W == FEW_BF16 && (!MakeMapBf16(&gate_up, p.gate_up, p.E * 2 * p.I, p.H, p.H, 128) || !MakeMapBf16(&down, p.down, p.E * p.H, p.I, p.I, 128))) return -2;
+  static bool configured[OGB_MAX_DEVICES] = {}, configured_down[OGB_MAX_DEVICES] = {};
+  if (!set_max_dyn_smem(few_gate_up_kernel<W>, int(FEW_SMEM_ONE), configured) || !set_max_dyn_smem(few_down_kernel<W>, FEW_DOWN_RING + 1024, configured_down)) return -3;
   static const int pdl = [] { const char* e = getenv("OGB_PDL"); return (e && e[0] == '0') ? 0 : 1; }();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -512,28 +533,33 @@ static int LaunchFew(const FewArgs& p, cudaStream_t stream) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(FEW_A_THREADS);
+  cfg.blockDim = dim3(FEW_THREADS);
   cfg.stream = stream;
   cfg.gridDim = dim3(FEW_CLUSTER);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  // As many clusters as run at once, two CTAs an SM or, with long rows, one.
+  // as many clusters as run at once
   static int clusters_at[OGB_MAX_DEVICES][2] = {};
-  const int two = smem <= FEW_SMEM_TWO;
   int dev = 0, clusters = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -4;
   const bool tracked = dev >= 0 && dev < OGB_MAX_DEVICES;
   if (tracked) clusters = clusters_at[dev][two];
   if (!clusters) {
-    cfg.dynamicSmemBytes = two ? FEW_SMEM_TWO : 227 * 1024;
+    cfg.dynamicSmemBytes = room;
     if (cudaOccupancyMaxActiveClusters(&clusters, few_gate_up_kernel<W>, &cfg) != cudaSuccess || clusters < 1) return -4;
     if (tracked) clusters_at[dev][two] = clusters;
   }
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = fixed + p.stages * STAGE;
   cfg.gridDim = dim3(unsigned(clusters * FEW_CLUSTER));
   cfg.numAttrs = pdl ? 2 : 1;
-  if (cudaLaunchKernelEx(&cfg, few_gate_up_kernel<W>, p) != cudaSuccess) return -4;
-  return launch_pdl(few_down_kernel<W>, dim3(unsigned((p.H + 15) / 16)), dim3(FEW_B_THREADS), 0, stream, p) ? 0 : -4;
+  if (cudaLaunchKernelEx(&cfg, few_gate_up_kernel<W>, gate_up, p) != cudaSuccess) return -4;
+  const int tiles = (p.H + 127) / 128;
+  p.splits = FEW_CLUSTER;
+  while (p.splits > 1 && tiles * p.splits > 2 * sm_count) p.splits /= 2;
+  attr[0].val.clusterDim = {unsigned(p.splits), 1, 1};
+  cfg.dynamicSmemBytes = FEW_DOWN_RING + 1024;
+  cfg.gridDim = dim3(unsigned(tiles * p.splits));
+  return cudaLaunchKernelEx(&cfg, few_down_kernel<W>, down, p) == cudaSuccess ? 0 : -4;
 }
 
 }  // namespace ogb
@@ -546,15 +572,16 @@ OGB_API long long ogb_moe_few_scratch_bytes(int T, int top, int I) {
 
 OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b,
                                const void* down, const void* down_b, void* out, int T, int H, int I, int E, int top, int rule, int weights, int act,
-                               float alpha, float limit, void* scratch, void* stream) {
+                               float alpha, float limit, void* scratch, int* status, int sm_count, void* stream) {
   if (ogb_moe_few_scratch_bytes(T, top, I) < 0 || !x || !router || !gate_up || !down || !out || !scratch || H < 1 || H % 8 || E < top || E > FEW_EXPERTS ||
       I % 64 || (weights != FEW_BF16 && H % 64) || rule < 0 || rule > 2 || weights < 0 || weights > 2 || (act != 1 && act != 2)) return -1;
   if ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * 2) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(scratch)) & 15)
     return -1;
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,
             static_cast<const __nv_bfloat16*>(gate_up_b), down, static_cast<const __nv_bfloat16*>(down_b), static_cast<__nv_bfloat16*>(out), T, H, I, E, top,
-            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan))};
+            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)), 0, 0, status};
+  if ((long long)E * 2 * I > 0x7fffffff || (long long)E * H > 0x7fffffff) return -5;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, s);
-  return weights == FEW_FP4_F16 ? LaunchFew<FEW_FP4_F16>(p, s) : LaunchFew<FEW_FP4_BF16>(p, s);
+  if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, sm_count, s);
+  return weights == FEW_FP4_F16 ? LaunchFew<FEW_FP4_F16>(p, sm_count, s) : LaunchFew<FEW_FP4_BF16>(p, sm_count, s);
 }

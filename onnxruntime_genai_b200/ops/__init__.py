@@ -1009,9 +1009,10 @@ def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, 
         x = x.clone(memory_format=torch.contiguous_format)
     out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
     scratch = torch.empty(_lib.lib().ogb_moe_few_scratch_bytes(T, top, I), dtype=torch.uint8, device=x.device)
-    _call_on(x.get_device(), "ogb_moe_few_tokens", x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),
+    ws = workspace(x.device)
+    _call_on(ws.index, "ogb_moe_few_tokens", x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),
              _ptr(gate_up_b), (down_w.packed if packed else down_w).data_ptr(), _ptr(down_b), out.data_ptr(), T, H, I, E, top, _FEW_RULES[weights],
-             (1 if gate_up_w.half else 2) if packed else 0, _FEW_ACTS[act], alpha, limit, scratch.data_ptr())
+             (1 if gate_up_w.half else 2) if packed else 0, _FEW_ACTS[act], alpha, limit, scratch.data_ptr(), ws.status, ws.sm_count)
     return out
 
 

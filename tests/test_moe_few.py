@@ -73,6 +73,6 @@ def test_launcher_refuses_on_the_host():
     L, A = _lib.lib(), 1 << 20
     assert L.ogb_moe_few_scratch_bytes(0, 2, 64) == -1 and L.ogb_moe_few_scratch_bytes(9, 2, 64) == -1 and L.ogb_moe_few_scratch_bytes(1, 33, 64) == -1
     call = lambda T=1, H=64, I=64, E=8, top=2, rule=0, weights=0, act=1: L.ogb_moe_few_tokens(A, 64, A, None, A, None, A, None, A, T, H, I, E, top, rule, weights, act, 1.0,
-                                                                                              0.0, A, None)
+                                                                                              0.0, A, None, 148, None)
     assert call(T=0) == -1 and call(T=9) == -1 and call(I=32) == -1 and call(E=1) == -1 and call(E=2000) == -1 and call(rule=3) == -1
     assert call(weights=3) == -1 and call(act=0) == -1 and call(H=68, weights=1) == -1 and call(H=0) == -1
