@@ -4,12 +4,13 @@
 // shared memory), so that each CTA can choose the experts, list those that any token meets, and go on to their gate and up rows without a kernel or a
 // grid barrier in between; the router is small beside the experts and comes from L2.  A warp computes eight features of one expert for all tokens: the
 // rows of an `mma.sync` tile of 16 are eight gate rows and the eight up rows of the same features, its columns the tokens, so that a thread holds a
-// gate and its up value and writes share * act(gate, up).
-// few_down_kernel: a CTA computes 16 columns of the output; its warps take equal parts of the sequence (expert, k) and are summed in warp order.
+// gate and its up value and writes share * act(gate, up).  The work of a cluster (items of 64 features, in steps of k) is cut into eight equal ranges; of an
+// item that a range border cuts, the later parts' sums go through memory to the CTA that began it.
+// few_down_kernel: a cluster computes 64 columns of the output; its CTAs, and two teams of warps in each, take equal parts of the sequence (expert, k); their
+// sums are sent to the CTA that finishes an output and added there in a fixed order.
 //
-// `mma.sync` is used on purpose: its eight columns are the eight tokens, and the operands go from memory to registers in the order in which they lie:
-// the k index of a product is permuted alike for both operands, so a lane's share of a row is one contiguous load.  A lane keeps several chunks of 64 k
-// values in flight, in a ring that runs on from one unit of work to the next.
+// `mma.sync` is used on purpose: its eight columns are the eight tokens, and weights go from shared memory to registers in the order in which they lie in
+// memory, with the k index of a product permuted alike for both operands.  A ring of bulk copies per CTA keeps some 100 KB an SM in flight.
 //
 // Roundings: the router's logits, all sums and the activation are fp32.  The activations times routing weights travel between the kernels in 16 bits (the
 // operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16, where values beyond 65504 become that.  The rows meet packed
@@ -22,12 +23,15 @@
 
 namespace ogb {
 
+template <int N> struct Int { static constexpr int value = N; };
 enum FewWeights : int { FEW_BF16 = 0, FEW_FP4_F16 = 1, FEW_FP4_BF16 = 2 };   // packed: the records of gemm_fp4.cu in their two forms
 constexpr int FEW_TOKENS = 8, FEW_TOP = 32, FEW_EXPERTS = 1024, FEW_MET = FEW_TOKENS * FEW_TOP;
 constexpr int FEW_CLUSTER = 8;
 constexpr int FEW_THREADS = 288, FEW_STAGES = 16;
 constexpr size_t FEW_SMEM_TWO = 112 * 1024, FEW_SMEM_ONE = 227 * 1024;          // shared memory of a CTA, with two or one on an SM
-constexpr int FEW_DOWN_RING = 72 * 1024;
+constexpr int FEW_DOWN_ROWS = 64, FEW_DOWN_RING = 96 * 1024, FEW_OUT = FEW_DOWN_ROWS * FEW_TOKENS;
+constexpr int FEW_MAX_CTAS = 320;                                               // of the first kernel: partial sums of a cut item, 4 KB each
+constexpr long long FEW_PREFETCH = 40 << 20;
 
 // What the first kernel leaves for the second.
 struct alignas(16) FewPlan {
@@ -52,74 +56,146 @@ struct FewArgs {
   int T, H, I, E, top, rule, act;
   float alpha, limit;
   FewPlan* plan;
+  float4* parts;        // [CTA][warp][lane] sums of the first kernel's cut items
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
   int stages, splits;   // of the first kernel's ring; CTAs of a cluster of the second
   int* status;
 };
 
 // ------------------------------------------------------------------------------- operands
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+// (volatile: they are for whole warps, and must not be moved into a branch that some lanes take)
+__device__ __forceinline__ void few_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  const uint32_t a[4] = {a0, a1, a2, a3};
-  mma_bf16_16816(d, a, b0, b1);
+__device__ __forceinline__ void few_mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// two mma of 16 k values each: a lane brings eight values of each of its rows (in pairs) and of its token
-__device__ __forceinline__ void mma_bf16_32(float (&d)[4], const uint4& r0, const uint4& r1, const uint4& b) {
-  mma_bf16_16816(d, r0.x, r1.x, r0.y, r1.y, b.x, b.y);
-  mma_bf16_16816(d, r0.z, r1.z, r0.w, r1.w, b.z, b.w);
+__device__ __forceinline__ void few_mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// A stage of the ring holds CHUNKS steps of 64 k values of a tile of 128 weight rows, as they lie in memory: packed records, or (bf16) a box of 64 columns with
-// the 128-byte swizzle.  A warp multiplies 16 of the rows, r0 = the row of lanes 4 g .. 4 g + 3 in the tile's first half of its 16, r1 in the second.
-template <int W>
+// 32 k values: a lane brings eight values of each of its rows (in pairs) and of its token; two sums, so that the two products do not wait for each other
+__device__ __forceinline__ void mma_bf16_32(float (&d)[2][4], const uint4& r0, const uint4& r1, const uint4& b) {
+  few_mma_bf16(d[0], r0.x, r1.x, r0.y, r1.y, b.x, b.y);
+  few_mma_bf16(d[1], r0.z, r1.z, r0.w, r1.w, b.z, b.w);
+}
+
+// Reads of shared memory by 32-bit address (volatile: they stay between the waits around them)
+template <int OFF> __device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4+%5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF> __device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2+%3];" : "=r"(v.x), "=r"(v.y) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF> __device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(OFF));
+  return v;
+}
+template <int OFF> __device__ __forceinline__ uint32_t lds8(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(OFF));
+  return v;
+}
+
+// A stage of the ring holds CHUNKS steps of 64 k values of a tile of ROWS weight rows, as they lie in memory: packed records (codes, then scales), or (bf16) a
+// box of 64 columns with the 128-byte swizzle.  A warp multiplies 16 of the rows: row r0 of the tile (lanes 4 g .. 4 g + 3) and row r1.
+template <int W, int ROWS>
 struct FewTile {
-  static constexpr int CHUNKS = W == FEW_BF16 ? 1 : 2;
-  static constexpr int BYTES = W == FEW_BF16 ? 128 * 128 : FP4_RECORD_BYTES;       // of a step
-  static __device__ __forceinline__ void mma(float (&acc)[4], const uint8_t* tile, int r0, int r1, int g, int q, const uint4 (&b)[2]) {
+  static constexpr int CHUNKS = W == FEW_BF16 && ROWS == 128 ? 1 : 2;
+  static constexpr int BYTES = W == FEW_BF16 ? ROWS * 128 : ROWS * 34;             // of a step
+  // Groups of warps that take turns at the stages.  A ring has a multiple of so many: a place of the ring belongs to one team, which then has seen every phase of its
+  // barrier (a team that came to a place whose stage before was another team's, and still on its way, would take the barrier's old parity for its own stage's).
+  static constexpr int TEAMS = 8 / (ROWS / 32);
+  static constexpr int ring(int room, int stage) { return (room / stage < FEW_STAGES ? room / stage : FEW_STAGES) / TEAMS * TEAMS; }
+  static constexpr int APART = ROWS == 128 ? 64 : 8, NEXT = ROWS == 128 ? 8 : 16;  // r1 - r0: gate and up rows, or eight rows on; the warp's second tile of 16
+  static constexpr float SCALE = W == FEW_FP4_F16 ? 0.015625f : 1.f;               // of the sums: the records hold a scale's code + 6
+  // a lane's place in a step: its part of row r0, and (packed) its scales
+  static __device__ __forceinline__ uint32_t place(int r0, int g, int q) { return W == FEW_BF16 ? r0 * 128 + ((q ^ g) << 4) : r0 * 32 + q * (W == FEW_FP4_F16 ? 8 : 4); }
+  static __device__ __forceinline__ uint32_t scales(int r0) { return ROWS * 32 + r0 * 2; }
+  // A step: every load, then every product.  at, sc: addresses of the lane's place and scales in it; b: the tokens' values
+  static __device__ __forceinline__ void mma(float (&acc)[2][4], uint32_t at, uint32_t sc, const uint4 (&b)[2]) {
     if constexpr (W == FEW_BF16) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int c = ((q + 4 * i) ^ g) << 4;
-        mma_bf16_32(acc, *reinterpret_cast<const uint4*>(tile + r0 * 128 + c), *reinterpret_cast<const uint4*>(tile + r1 * 128 + c), b[i]);
-      }
-    } else if constexpr (W == FEW_FP4_F16) {
-      const uint2 q0 = *reinterpret_cast<const uint2*>(tile + r0 * 32 + q * 8), q1 = *reinterpret_cast<const uint2*>(tile + r1 * 32 + q * 8);
-      const uint32_t s0 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r0 * 2), s1 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r1 * 2);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {                       // a block of 32 has one scale per row (the records hold code + 6): its sum is scaled as a whole
-        uint32_t u[4], v[4];
-        cvt_e2m1x8_f16(i ? q0.y : q0.x, u);
-        cvt_e2m1x8_f16(i ? q1.y : q1.x, v);
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        mma_f16_16816(t, u[0], v[0], u[1], v[1], b[i].x, b[i].y);
-        mma_f16_16816(t, u[2], v[2], u[3], v[3], b[i].z, b[i].w);
-        const float f0 = __uint_as_float(((i ? s0 >> 8 : s0 & 255u) - 6u) << 23), f1 = __uint_as_float(((i ? s1 >> 8 : s1 & 255u) - 6u) << 23);
-        acc[0] = fmaf(t[0], f0, acc[0]);
-        acc[1] = fmaf(t[1], f0, acc[1]);
-        acc[2] = fmaf(t[2], f1, acc[2]);
-        acc[3] = fmaf(t[3], f1, acc[3]);
-      }
-    } else {
-      const uint32_t s0 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r0 * 2), s1 = *reinterpret_cast<const uint16_t*>(tile + 128 * 32 + r1 * 2);
+      uint4 a[2][2][2];                                                            // [tile of 16][half of the step][row]
+      const uint32_t x = at ^ 64u;                                                 // places 4 and more of a row's eight: (q + 4) ^ g
+      a[0][0][0] = lds128<0>(at);
+      a[0][0][1] = lds128<APART * 128>(at);
+      a[0][1][0] = lds128<0>(x);
+      a[0][1][1] = lds128<APART * 128>(x);
+      a[1][0][0] = lds128<NEXT * 128>(at);
+      a[1][0][1] = lds128<(NEXT + APART) * 128>(at);
+      a[1][1][0] = lds128<NEXT * 128>(x);
+      a[1][1][1] = lds128<(NEXT + APART) * 128>(x);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        mma_bf16_32(acc, deq_fp4_word_bf16(*reinterpret_cast<const uint32_t*>(tile + r0 * 32 + i * 16 + q * 4), i ? s0 >> 8 : s0 & 255u),
-                    deq_fp4_word_bf16(*reinterpret_cast<const uint32_t*>(tile + r1 * 32 + i * 16 + q * 4), i ? s1 >> 8 : s1 & 255u), b[i]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          few_mma_bf16(acc[m], a[m][i][0].x, a[m][i][1].x, a[m][i][0].y, a[m][i][1].y, b[i].x, b[i].y);
+          few_mma_bf16(acc[m], a[m][i][0].z, a[m][i][1].z, a[m][i][0].w, a[m][i][1].w, b[i].z, b[i].w);
+        }
+    } else if constexpr (W == FEW_FP4_F16) {
+      const uint2 q00 = lds64<0>(at), q01 = lds64<APART * 32>(at), q10 = lds64<NEXT * 32>(at), q11 = lds64<(NEXT + APART) * 32>(at);
+      const uint32_t f[2][2][2] = {{{lds8<0>(sc), lds8<1>(sc)}, {lds8<APART * 2>(sc), lds8<APART * 2 + 1>(sc)}},
+                                   {{lds8<NEXT * 2>(sc), lds8<NEXT * 2 + 1>(sc)}, {lds8<(NEXT + APART) * 2>(sc), lds8<(NEXT + APART) * 2 + 1>(sc)}}};
+      float t[2][2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                     // a block of 32 has one scale per row: its sum is scaled as a whole
+          uint32_t u[4], v[4];
+          cvt_e2m1x8_f16(i ? (m ? q10.y : q00.y) : (m ? q10.x : q00.x), u);
+          cvt_e2m1x8_f16(i ? (m ? q11.y : q01.y) : (m ? q11.x : q01.x), v);
+          few_mma_f16_first(t[m][i], u[0], v[0], u[1], v[1], b[i].x, b[i].y);
+          few_mma_f16(t[m][i], u[2], v[2], u[3], v[3], b[i].z, b[i].w);
+        }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float x0 = __uint_as_float(f[m][0][i] << 23), x1 = __uint_as_float(f[m][1][i] << 23);
+          acc[m][0] = fmaf(t[m][i][0], x0, acc[m][0]);
+          acc[m][1] = fmaf(t[m][i][1], x0, acc[m][1]);
+          acc[m][2] = fmaf(t[m][i][2], x1, acc[m][2]);
+          acc[m][3] = fmaf(t[m][i][3], x1, acc[m][3]);
+        }
+    } else {
+      auto half = [&](auto i, auto m) {
+        constexpr int I_ = decltype(i)::value, R = decltype(m)::value * NEXT;
+        const uint4 a0 = deq_fp4_word_bf16(lds32<R * 32 + I_ * 16>(at), lds8<R * 2 + I_>(sc));
+        const uint4 a1 = deq_fp4_word_bf16(lds32<(R + APART) * 32 + I_ * 16>(at), lds8<(R + APART) * 2 + I_>(sc));
+        few_mma_bf16(acc[R ? 1 : 0], a0.x, a1.x, a0.y, a1.y, b[I_].x, b[I_].y);
+        few_mma_bf16(acc[R ? 1 : 0], a0.z, a1.z, a0.w, a1.w, b[I_].z, b[I_].w);
+      };
+      half(Int<0>{}, Int<0>{});
+      half(Int<0>{}, Int<1>{});
+      half(Int<1>{}, Int<0>{});
+      half(Int<1>{}, Int<1>{});
+    }
+  }
+  // Copies n steps from `chunk` on of rows row .. row + ROWS - 1 of expert e to a stage, counted in bytes on its barrier; by one thread.
+  static __device__ __forceinline__ void copy(uint8_t* dst, uint64_t* bar, const CUtensorMap* map, const void* packed, int e, int row, int chunk, int n, int N, int K) {
+    if constexpr (W == FEW_BF16) {
+      for (int j = 0; j < n; ++j) tma_load_2d(dst + j * BYTES, map, bar, (chunk + j) * 64, e * N + row);
+    } else {
+      const int tiles = (N + 127) >> 7;
+      const uint8_t* rec = static_cast<const uint8_t*>(packed) + (((long long)e * (K >> 6) + chunk) * tiles + (row >> 7)) * FP4_RECORD_BYTES;
+      for (int j = 0; j < n; ++j, rec += (long long)tiles * FP4_RECORD_BYTES) {
+        if constexpr (ROWS == 128) {
+          bulk_copy_g2s(dst + j * BYTES, rec, FP4_RECORD_BYTES, bar);
+        } else {
+          bulk_copy_g2s(dst + j * BYTES, rec + (row & 127) * 32, ROWS * 32, bar);
+          bulk_copy_g2s(dst + j * BYTES + ROWS * 32, rec + 128 * 32 + (row & 127) * 2, ROWS * 2, bar);
+        }
+      }
     }
   }
 };
-// Copies step `chunk` of 128 weight rows (tile `tile` of expert e's rows) to shared memory; by one thread.
-template <int W>
-__device__ __forceinline__ void few_copy(uint8_t* dst, uint64_t* bar, const CUtensorMap* map, const void* packed, int e, int tile, int chunk, int N, int K) {
-  if constexpr (W == FEW_BF16) {
-    tma_load_2d(dst, map, bar, chunk * 64, e * N + tile * 128);
-  } else {
-    const int tiles = (N + 127) >> 7;
-    bulk_copy_g2s(dst, static_cast<const uint8_t*>(packed) + (((long long)e * (K >> 6) + chunk) * tiles + tile) * FP4_RECORD_BYTES, FP4_RECORD_BYTES, bar);
-  }
-}
 
 // Eight 16-bit values in the order in which a lane's eight weights of a row come out of their load: pairs (0, 1) (2, 3) .. or, from records in fp16 form,
 // (0, 4) (1, 5) (2, 6) (3, 7).
@@ -133,34 +209,67 @@ __device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // 
 // ------------------------------------------------------------------------------- ring of copies
 // Warp 8 copies, warps 0 .. 7 multiply.  All waits are bounded; after a failed one every warp leaves its loop.
 struct FewBars { uint64_t full[FEW_STAGES], empty[FEW_STAGES]; int abort; };
-__device__ __forceinline__ void few_init(FewBars& b, int stages) {
-  for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], 1); mbar_init(&b.empty[s], 8); }
+__device__ __forceinline__ void few_init(FewBars& b, int stages, int warps) {      // warps that read a stage
+  for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], 1); mbar_init(&b.empty[s], warps); }
   b.abort = 0;
   mbar_fence_init();
 }
-struct FewRing {
+struct FewRing {                       // the copying side
   int stages, s = 0, filled = 0;
   uint32_t ph = 0;
   __device__ __forceinline__ void next() {
     ++filled;
     if (++s == stages) { s = 0; ph ^= 1; }
   }
-  __device__ __forceinline__ bool fail(FewBars& b, int* status) { atomicMax(status, OGB_ERR_WAIT_TMA); *reinterpret_cast<volatile int*>(&b.abort) = 1; return false; }
   __device__ __forceinline__ bool wait_empty(FewBars& b, int* status) {
-    if (filled < stages) return true;
-    return __all_sync(0xffffffffu, mbar_wait_bounded(&b.empty[s], ph ^ 1, &b.abort)) || fail(b, status);
-  }
-  // A consumer warp hands the stage before this one back only here.  Directly behind the products of its own stage the arrival could overtake reads of shared
-  // memory that are still on their way (the compiler may put it in front of the products that wait for them; seen as single wrong rows); behind the wait for the
-  // next stage all products, and so all reads, have been issued and answered.
-  __device__ __forceinline__ bool wait_full(FewBars& b, int* status, int lane) {
-    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&b.full[s], ph, &b.abort))) return fail(b, status);
-    if (filled > 0 && lane == 0) mbar_arrive(&b.empty[(s == 0 ? stages : s) - 1]);
-    return true;
+    if (filled < stages || __all_sync(0xffffffffu, mbar_wait_bounded(&b.empty[s], ph ^ 1, &b.abort))) return true;
+    atomicMax(status, OGB_ERR_WAIT_TMA);
+    *reinterpret_cast<volatile int*>(&b.abort) = 1;
+    return false;
   }
   __device__ __forceinline__ void drain(FewBars& b) {          // copies in flight still write shared memory: give them time to land
     volatile int never = 0;
     for (int i = max(0, filled - stages); i < filled; ++i) mbar_wait_bounded(&b.full[i % stages], (i / stages) & 1, &never, 200000000ull);
+  }
+};
+static __device__ __noinline__ bool few_wait_slow(FewBars* b, uint32_t full, uint32_t ph, int* status) {
+  const uint64_t t0 = global_timer_ns();
+  uint32_t spins = 0, ok = 0;
+  while (!ok) {
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(full), "r"(ph) : "memory");
+    if (!ok && (++spins & 0x3ff) == 0 && (*reinterpret_cast<volatile int*>(&b->abort) || global_timer_ns() - t0 > 2000000000ull)) break;
+  }
+  if (__all_sync(0xffffffffu, ok != 0)) return true;
+  atomicMax(status, OGB_ERR_WAIT_TMA);
+  *reinterpret_cast<volatile int*>(&b->abort) = 1;
+  return false;
+}
+template <int STAGE>
+struct FewReader {                     // the multiplying side
+  FewBars* b;
+  uint32_t base, data, full, last = 0, ph = 0, end;      // addresses: first stage, this stage, its barrier, the barrier of the stage read before; end of the ring
+  __device__ __forceinline__ FewReader(FewBars* bars, const void* ring, int stages)
+      : b(bars), base(smem_u32(ring)), data(base), full(smem_u32(bars->full)), end(base + stages * STAGE) {}
+  __device__ __forceinline__ void next() {
+    data += STAGE;
+    full += 8;
+    if (data == end) { data = base; full = smem_u32(b->full); ph ^= 1; }
+  }
+  // false: the wait ran out; the warp goes through its loop without reading, so that it meets the barriers that the others wait at
+  __device__ __forceinline__ bool wait(int* status) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(full), "r"(ph) : "memory");
+    if (!__all_sync(0xffffffffu, ok) && !few_wait_slow(b, full, ph, status)) return false;
+    last = full + sizeof(uint64_t) * FEW_STAGES;         // (the stage's `empty`)
+    return true;
+  }
+  // Hands back the stage that this warp has read; called in the next turn of the loop.  Directly behind its products the arrival could overtake reads of shared memory
+  // that are still on their way (seen as single wrong rows: nothing makes the arrival wait for loads whose values are used later); a turn later the products have
+  // been issued, for which all their operands had to be there.
+  __device__ __forceinline__ void release(int lane) {
+    __syncwarp();
+    if (last && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(last) : "memory");
+    last = 0;
   }
 };
 
@@ -168,6 +277,7 @@ struct FewRing {
 // Shared memory of the first kernel.
 struct FewShared {
   FewBars bars;
+  float4 teams[2][4][64];             // [item][warp][half of its rows, lane] sums of the second team
   float red[FEW_THREADS / 32][16 * FEW_TOKENS];
   uint32_t top[FEW_TOKENS];          // bits of the rows' largest magnitudes
   uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
@@ -183,21 +293,26 @@ __device__ __forceinline__ uint32_t few_key(float v) {
   return v != v ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 // Choice of `top` experts for a token by one warp: the largest logits, the lowest index among equal ones; a token whose logits are not numbers takes
-// expert 0.  A lane holds every 32nd expert and looks for its best one anew only when that was taken.
+// expert 0.  A lane holds every 32nd expert, up to 32 R, and looks for its best one anew only when that was taken.
+template <int R>
 __device__ __forceinline__ void few_choose(const float* row, int E, int top, int rule, int lane, int& id, float& share) {
-  uint32_t taken = 0, best = 0;      // taken, bit i: expert lane + 32 i
-  int at = 0x7fffffff;
+  uint32_t key[R];                   // 0: nothing to choose
   bool bad = false;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const float v = i * 32 + lane < E ? row[i * 32 + lane] : -INFINITY;
+    key[i] = i * 32 + lane < E ? few_key(v) : 0u;
+    bad |= v != v;
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  uint32_t best = 0;
+  int at = 0x7fffffff;
   auto scan = [&]() {
     best = 0;
     at = 0x7fffffff;
-    for (int i = 0, e = lane; e < E; ++i, e += 32) {
-      const uint32_t k = taken >> i & 1 ? 0u : few_key(row[e]);
-      if (k > best) { best = k; at = e; }
-    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) if (key[i] > best) { best = key[i]; at = i * 32 + lane; }
   };
-  for (int e = lane; e < E; e += 32) bad |= row[e] != row[e];
-  bad = __any_sync(0xffffffffu, bad);
   scan();
   float most = 0.f, mine = 0.f;
   id = 0;
@@ -207,7 +322,11 @@ __device__ __forceinline__ void few_choose(const float* row, int E, int top, int
     const float v = __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
     if (j == 0) most = v;
     if (lane == j) { mine = v; id = k ? e : 0; }
-    if (k && at == e) { taken |= 1u << (e >> 5); scan(); }
+    if (k && at == e) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) if (i == e >> 5) key[i] = 0;
+      scan();
+    }
   }
   const float w = lane < top ? expf(mine - most) : 0.f;
   float sum = warp_sum(w);
@@ -221,7 +340,7 @@ __device__ __forceinline__ void few_choose(const float* row, int E, int top, int
 
 template <int W>
 __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
-  using Tile = FewTile<W>;
+  using Tile = FewTile<W, 128>;
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -234,45 +353,54 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the others' shared memory is written only once they run
   for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) sh.mask[e] = 0;
   if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
-  if (threadIdx.x == 0) few_init(sh.bars, p.stages);
+  if (threadIdx.x == 0) few_init(sh.bars, p.stages, 8 / Tile::TEAMS);
+  __syncwarp();
   __syncthreads();
-  pdl_wait();
-  pdl_launch_dependents();
 
-  // the largest magnitude of every row, where the rows are to be scaled: a warp takes 256 values of a token at a time
+  // The rows: a warp takes 256 values of a token at a time and keeps the first pieces in registers until the rows' largest magnitudes are known (packed experts:
+  // fp16 after a scaling).
+  constexpr int HELD = 6, WARPS = FEW_THREADS / 32;
   const int parts = (Hp + 255) >> 8, pieces = p.T * parts;
+  auto piece = [&](int i) {
+    const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
+    return i < pieces && k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 held[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) held[h] = piece(warp + h * WARPS);
   if (W == FEW_FP4_F16) {
-#pragma unroll 4
-    for (int i = warp; i < pieces; i += FEW_THREADS / 32) {
-      const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
-      const uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+    auto largest = [&](int i, const uint4& v) {
+      if (i >= pieces) return;
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) top = max(top, max(w[j] << 16 & 0x7fffffffu, w[j] & 0x7fff0000u));
       top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) atomicMax(&sh.top[t], top);
-    }
+      if (lane == 0) atomicMax(&sh.top[i / parts], top);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) largest(warp + h * WARPS, held[h]);
+    for (int i = warp + HELD * WARPS; i < pieces; i += WARPS) largest(i, piece(i));
   }
 
   // router logits of this CTA's experts: 16 experts x 8 tokens at a time, the warps share k
   const int per = (p.E + FEW_CLUSTER - 1) / FEW_CLUSTER, e_end = min(p.E, (rank + 1) * per);
   bool met_cluster = false;
   for (int e0 = rank * per; e0 < (rank + 1) * per; e0 += 16) {               // (the same number of rounds in every CTA)
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[2][4] = {};
     const bool r0 = e0 + g < e_end, r1 = e0 + g + 8 < e_end;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const __nv_bfloat16* w0 = p.router + (long long)(r0 ? e0 + g : 0) * p.H;
     const __nv_bfloat16* w1 = p.router + (long long)(r1 ? e0 + g + 8 : 0) * p.H;
-#pragma unroll 4
+#pragma unroll 5
     for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += FEW_THREADS) {
       const bool in = k < p.H;
       const uint4 a0 = r0 && in ? *reinterpret_cast<const uint4*>(w0 + k) : zero, a1 = r1 && in ? *reinterpret_cast<const uint4*>(w1 + k) : zero;
       const uint4 b = g < p.T && in ? *reinterpret_cast<const uint4*>(p.x + g * p.ldx + k) : zero;
       mma_bf16_32(acc, a0, a1, b);
     }
-    *reinterpret_cast<float2*>(&sh.red[warp][g * 8 + q * 2]) = make_float2(acc[0], acc[1]);
-    *reinterpret_cast<float2*>(&sh.red[warp][(g + 8) * 8 + q * 2]) = make_float2(acc[2], acc[3]);
+    *reinterpret_cast<float2*>(&sh.red[warp][g * 8 + q * 2]) = make_float2(acc[0][0] + acc[1][0], acc[0][1] + acc[1][1]);
+    *reinterpret_cast<float2*>(&sh.red[warp][(g + 8) * 8 + q * 2]) = make_float2(acc[0][2] + acc[1][2], acc[0][3] + acc[1][3]);
     __syncthreads();
     if (!met_cluster) { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); met_cluster = true; }
     if (threadIdx.x < 128) {
@@ -289,27 +417,34 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     }
     __syncthreads();
   }
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   // the rows as the products read them
-#pragma unroll 4
-  for (int i = warp; i < pieces; i += FEW_THREADS / 32) {
+  auto put = [&](int i, uint4 v) {
     const int t = i / parts, k = (i - t * parts) * 256 + lane * 8;
-    uint4 v = k < p.H ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+    if (i >= pieces || k >= Hp) return;
     if (W == FEW_FP4_F16) {
       const float scale = __uint_as_float(uint32_t(few_shift(sh.top[t]) + 127) << 23);
       const float2 a = unpack_bf16x2(v.x), b = unpack_bf16x2(v.y), c = unpack_bf16x2(v.z), d = unpack_bf16x2(v.w);
       v = make_uint4(pack_f16x2(a.x * scale, c.x * scale), pack_f16x2(a.y * scale, c.y * scale), pack_f16x2(b.x * scale, d.x * scale),
                      pack_f16x2(b.y * scale, d.y * scale));
     }
-    if (k < Hp) *reinterpret_cast<uint4*>(xs + t * xs_ld + k) = v;
-  }
+    *reinterpret_cast<uint4*>(xs + t * xs_ld + k) = v;
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) put(warp + h * WARPS, held[h]);
+  for (int i = warp + HELD * WARPS; i < pieces; i += WARPS) put(i, piece(i));
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 
   // choices, and the experts that any token meets
   if (warp < p.T) {
     int id;
     float share;
-    few_choose(logits + warp * p.E, p.E, p.top, p.rule, lane, id, share);
+    const float* row = logits + warp * p.E;
+    if (p.E <= 128) few_choose<4>(row, p.E, p.top, p.rule, lane, id, share);
+    else if (p.E <= 256) few_choose<8>(row, p.E, p.top, p.rule, lane, id, share);
+    else few_choose<32>(row, p.E, p.top, p.rule, lane, id, share);
     if (lane < p.top) {
       sh.plan.ids[warp * p.top + lane] = id;
       sh.plan.share[warp * p.top + lane] = share;
@@ -340,84 +475,164 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_THREADS) reinterpret_cast<uint4*>(p.plan)[i] = src[i];
   }
 
-  // gate and up rows: an item is 64 features of a met expert, 128 rows that lie together; a warp takes eight features
-  const int tiles = p.I >> 6, items = sh.plan.met * tiles, chunks = Hp >> 6;
+  // Gate and up rows: an item is 64 features of a met expert, 128 rows that lie together; a warp takes eight features.  The clusters share the items, the CTAs
+  // of a cluster the steps of its items.
+  const int tiles = p.I >> 6, items = sh.plan.met * tiles, chunks = Hp >> 6, steps = (chunks + Tile::CHUNKS - 1) / Tile::CHUNKS;
+  const unsigned clusters = gridDim.x / FEW_CLUSTER, cluster = blockIdx.x / FEW_CLUSTER;
+  const int item0 = int(unsigned(items) * cluster / clusters), mine = int(unsigned(items) * (cluster + 1) / clusters) - item0;
+  const unsigned all_steps = unsigned(mine * steps);
+  const int lo = int(all_steps * rank / FEW_CLUSTER), hi = int(all_steps * (rank + 1) / FEW_CLUSTER);
+  // Activations of 16 features x 2 tokens a lane: acc[m] the sums of features m * 8 + g of the warp's 16 (gate, gate, up, up)
+  auto finish = [&](int item, const float (&acc)[2][4]) {
+    const int d = item / tiles, f0 = (item - d * tiles) * 64 + (warp & 3) * 16;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const long long row = (long long)sh.plan.expert[d] * 2 * p.I + (f0 >> 6) * 128 + (f0 & 63) + m * 8 + g;
+      const float bg = p.gate_up_b ? bf2f(p.gate_up_b[row]) : 0.f, bu = p.gate_up_b ? bf2f(p.gate_up_b[row + 64]) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = q * 2 + j, slot = sh.plan.slot[d][t];
+        if (slot == 255) continue;
+        const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) * Tile::SCALE : 1.f;
+        float gate = fmaf(acc[m][j], s, bg), up = fmaf(acc[m][2 + j], s, bu), v = gate;
+        if (p.act == 2) {
+          if (p.limit > 0.f) {             // (comparisons, not minima: what is not a number stays that)
+            gate = gate > p.limit ? p.limit : gate;
+            up = up > p.limit ? p.limit : up < -p.limit ? -p.limit : up;
+          }
+          v = p.alpha * gate;
+          up += 1.f;
+        }
+        const int pair = t * p.top + slot;
+        v = gate / (1.f + expf(-v)) * up * sh.plan.share[pair];
+        p.h[(long long)pair * p.I + f0 + m * 8 + few_place<W>(g)] = uint16_t(W == FEW_FP4_F16 ? f16x2_sat(v, 0.f) : pack_bf16x2(v, 0.f));
+      }
+    }
+  };
+  const int last_item = hi > lo ? (hi - 1) / steps : 0;
+  const bool open_end = hi > lo && hi % steps != 0 && last_item * steps >= lo;        // began here, ends elsewhere: finished below
+  float left[2][4] = {};                               // its sums
   if (warp == 8) {
     FewRing r{p.stages};
     bool ok = true;
-    for (int item = blockIdx.x; item < items && ok; item += gridDim.x) {
-      const int e = sh.plan.expert[item / tiles], tile = item % tiles;
-      for (int c = 0; c < chunks; c += Tile::CHUNKS) {
-        ok = r.wait_empty(sh.bars, p.status);
-        if (!ok) break;
-        if (elect_one()) {
-          const int n = min(Tile::CHUNKS, chunks - c);
-          uint64_t* bar = &sh.bars.full[r.s];
-          mbar_expect_tx(bar, n * Tile::BYTES);
-          for (int i = 0; i < n; ++i) few_copy<W>(ring + r.s * STAGE + i * Tile::BYTES, bar, &map, p.gate_up, e, tile, c + i, 2 * p.I, p.H);
-        }
-        __syncwarp();
-        r.next();
+    const int item = lo / steps;
+    int c = (lo - item * steps) * Tile::CHUNKS, d = (item0 + item) / tiles, tile = item0 + item - d * tiles;
+    for (int i = lo; i < hi; ++i) {
+      ok = r.wait_empty(sh.bars, p.status);
+      if (!ok) break;
+      const int n = min(Tile::CHUNKS, chunks - c);
+      uint64_t* bar = &sh.bars.full[r.s];
+      if (elect_one()) {
+        mbar_expect_tx(bar, n * Tile::BYTES);
+        Tile::copy(ring + r.s * STAGE, bar, &map, p.gate_up, sh.plan.expert[d], tile * 128, c, n, 2 * p.I, p.H);
+      }
+      __syncwarp();
+      r.next();
+      c += Tile::CHUNKS;
+      if (c >= chunks) {
+        c = 0;
+        if (++tile == tiles) { tile = 0; ++d; }
       }
     }
     if (!ok) r.drain(sh.bars);
-    return;
-  }
-  FewRing r{p.stages};
-  const uint16_t* xt = xs + (g < p.T ? g : 0) * xs_ld + q * 8;           // (columns beyond the tokens: any numbers, they are not looked at)
-  const int r0 = warp * 8 + g;
-  for (int item = blockIdx.x; item < items; item += gridDim.x) {
-    const int d = item / tiles, tile = item - d * tiles, e = sh.plan.expert[d], i0 = tile * 64 + warp * 8;
-    const long long row = (long long)e * 2 * p.I + tile * 128 + r0;
-    const float bg = p.gate_up_b ? bf2f(p.gate_up_b[row]) : 0.f, bu = p.gate_up_b ? bf2f(p.gate_up_b[row + 64]) : 0.f;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < chunks; c += Tile::CHUNKS) {
-      if (!r.wait_full(sh.bars, p.status, lane)) return;
-#pragma unroll
-      for (int i = 0; i < Tile::CHUNKS; ++i) {
-        if (i > 0 && c + i >= chunks) break;
-        const uint4 b[2] = {*reinterpret_cast<const uint4*>(xt + (c + i) * 64), *reinterpret_cast<const uint4*>(xt + (c + i) * 64 + 32)};
-        Tile::mma(acc, ring + r.s * STAGE + i * Tile::BYTES, r0, r0 + 64, g, q, b);
+    // While the rest of this kernel runs, memory is idle: where the met experts' down rows are few enough to stay in L2, they are fetched there
+    const long long per_expert = W == FEW_BF16 ? (long long)p.H * p.I * 2 : (long long)(p.I >> 6) * ((p.H + 127) >> 7) * FP4_RECORD_BYTES;
+    if (per_expert * sh.plan.met <= FEW_PREFETCH) {
+      constexpr int PIECE = 16384;
+      const int per = int((per_expert + PIECE - 1) / PIECE), all = per * sh.plan.met;
+      for (int i = int(blockIdx.x) * 32 + lane; i < all; i += int(gridDim.x) * 32) {
+        const int d = i / per;
+        const long long at = (long long)(i - d * per) * PIECE;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                     ::"l"(static_cast<const uint8_t*>(p.down) + per_expert * sh.plan.expert[d] + at), "r"(uint32_t(min((long long)PIECE, per_expert - at))) : "memory");
+      }
+    }
+  } else {
+    const uint32_t xt = smem_u32(xs + (g < p.T ? g : 0) * xs_ld + q * 8);    // (columns beyond the tokens: any numbers, they are not looked at)
+    const int team = warp >> 2;
+    const uint32_t place = Tile::place((warp & 3) * 16 + g, g, q), scales = Tile::scales((warp & 3) * 16 + g);
+    float acc[2][4] = {};
+    FewReader<STAGE> r(&sh.bars, ring, p.stages);
+    int item = lo / steps, c = (lo - item * steps) * Tile::CHUNKS, parity = 0;
+    bool whole = c == 0, ok = true;
+    for (int i = lo; i < hi; ++i, parity ^= 1) {
+      r.release(lane);
+      if (parity == team && ok && (ok = r.wait(p.status))) {
+        const uint32_t x = xt + c * 128;
+        uint4 b[2] = {lds128<0>(x), lds128<64>(x)};
+        Tile::mma(acc, r.data + place, r.data + scales, b);
+        if (Tile::CHUNKS == 2 && c + 1 < chunks) {
+          b[0] = lds128<128>(x);
+          b[1] = lds128<192>(x);
+          Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+        }
       }
       r.next();
-    }
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int t = q * 2 + j, slot = sh.plan.slot[d][t];
-      if (slot == 255) continue;
-      const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) : 1.f;
-      float gate = fmaf(acc[j], s, bg), up = fmaf(acc[2 + j], s, bu), v = gate;
-      if (p.act == 2) {
-        if (p.limit > 0.f) {             // (comparisons, not minima: what is not a number stays that)
-          gate = gate > p.limit ? p.limit : gate;
-          up = up > p.limit ? p.limit : up < -p.limit ? -p.limit : up;
-        }
-        v = p.alpha * gate;
-        up += 1.f;
+      c += Tile::CHUNKS;
+      if (c < chunks && i + 1 < hi) continue;
+      // The item's part in this range is done: the second team's sums go to the first, which finishes the item, leaves a part of it to the CTA that began it, or
+      // keeps what it has until the others' parts are there.  Two buffers: a team is at most one item ahead of the other.
+      float4* mine_ = sh.teams[item & 1][warp & 3];
+      if (team == 1) {
+        mine_[lane] = make_float4(acc[0][0], acc[0][1], acc[0][2], acc[0][3]);
+        mine_[32 + lane] = make_float4(acc[1][0], acc[1][1], acc[1][2], acc[1][3]);
       }
-      const int pair = t * p.top + slot;
-      v = gate / (1.f + expf(-v)) * up * sh.plan.share[pair];
-      p.h[(long long)pair * p.I + i0 + few_place<W>(g)] = uint16_t(W == FEW_FP4_F16 ? f16x2_sat(v, 0.f) : pack_bf16x2(v, 0.f));
+      __syncwarp();                                    // (lanes may still be apart behind the last item's activations: barriers want whole warps)
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (team == 0) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const float4 v = mine_[m * 32 + lane];
+          acc[m][0] += v.x; acc[m][1] += v.y; acc[m][2] += v.z; acc[m][3] += v.w;
+        }
+        if (!whole) {
+          for (int m = 0; m < 2; ++m) p.parts[((blockIdx.x * 4 + warp) * 2 + m) * 32 + lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+        } else if (c >= chunks) {
+          finish(item0 + item, acc);
+        } else {
+          for (int m = 0; m < 2; ++m) for (int j = 0; j < 4; ++j) left[m][j] = acc[m][j];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[0][j] = acc[1][j] = 0.f;
+      c = 0;
+      whole = true;
+      ++item;
     }
+  }
+  __syncwarp();
+  cluster_sync_all();                                    // the cluster's partial sums are in memory
+  if (warp < 4 && open_end) {
+    const int end = (last_item + 1) * steps;             // ranges behind this one, up to the item's end, in order
+    for (int o = rank + 1; o < FEW_CLUSTER; ++o) {
+      const int from = int(all_steps * o / FEW_CLUSTER);
+      if (from >= end) break;
+      const int to = int(all_steps * (o + 1) / FEW_CLUSTER);
+      if (from == to) continue;
+      for (int m = 0; m < 2; ++m) {
+        const float4 v = __ldcg(&p.parts[(((cluster * FEW_CLUSTER + o) * 4 + warp) * 2 + m) * 32 + lane]);
+        left[m][0] += v.x; left[m][1] += v.y; left[m][2] += v.z; left[m][3] += v.w;
+      }
+    }
+    finish(item0 + last_item, left);
   }
 }
 
-// A cluster computes 128 columns of the output, its CTAs take equal parts of the sequence (expert, k); partial sums are sent to the CTA that finishes their rows.
 template <int W>
 __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
-  using Tile = FewTile<W>;
+  using Tile = FewTile<W, FEW_DOWN_ROWS>;
   constexpr int H_LD = Tile::CHUNKS * 128 + 64, H_OFF = Tile::CHUNKS * Tile::BYTES, STAGE = (H_OFF + FEW_TOKENS * H_LD + 1023) / 1024 * 1024;
-  constexpr int STAGES = FEW_DOWN_RING / STAGE < FEW_STAGES ? FEW_DOWN_RING / STAGE : FEW_STAGES;
+  constexpr int STAGES = Tile::ring(FEW_DOWN_RING, STAGE), TEAMS = Tile::TEAMS;
+  static_assert(STAGES >= TEAMS, "a place for every team");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ FewBars bars;
-  __shared__ __align__(16) FewPlan plan;
-  __shared__ __align__(16) float red[128 * FEW_TOKENS];                         // [sender][rows of this CTA: 128 / splits][token]
+  __shared__ FewPlan plan;
+  __shared__ __align__(16) float red[TEAMS * (FEW_OUT + 2 * FEW_CLUSTER)];     // [sender: CTA, team][outputs of this CTA]
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int rank = int(cluster_ctarank()), splits = p.splits, tile = blockIdx.x / splits;
+  const int rank = int(cluster_ctarank()), splits = p.splits, n0 = int(blockIdx.x) / splits * FEW_DOWN_ROWS;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (threadIdx.x == 0) few_init(bars, STAGES);
-  pdl_wait();
+  if (threadIdx.x == 0) few_init(bars, STAGES, 8 / TEAMS);
   pdl_launch_dependents();
   {
     const uint4* src = reinterpret_cast<const uint4*>(p.plan);
@@ -425,29 +640,43 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
   }
   __syncthreads();
   const int chunks = p.I >> 6, steps = (chunks + Tile::CHUNKS - 1) / Tile::CHUNKS, total = plan.met * steps;
-  const int lo = int((long long)total * rank / splits), hi = int((long long)total * (rank + 1) / splits);
+  const int lo = int(unsigned(total) * rank / splits), hi = int(unsigned(total) * (rank + 1) / splits);
+  // outputs [row of the tile][token], dealt out to the cluster's CTAs in runs of `per`
+  const int per = ((FEW_OUT + splits - 1) / splits + 1) & ~1, first = rank * per, last = min(FEW_OUT, first + per);
+  auto output = [&](int i, int& n, int& t) {
+    n = n0 + (first + i) / FEW_TOKENS;
+    t = (first + i) % FEW_TOKENS;
+    return first + i < last && n < p.H && t < p.T;
+  };
+  float bias[2] = {0.f, 0.f};                          // of this thread's outputs, fetched while the first stages are on their way
+  if (p.down_b) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int n, t;
+      if (output(int(threadIdx.x) + k * FEW_THREADS, n, t))
+        for (int j = 0; j < p.top; ++j) bias[k] += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
+    }
+  }
   bool ok = true;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  float sum[2][4] = {};
+  const int team = warp >> 1, r0 = (warp & 1) * 32 + g;
+  int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
   if (warp == 8) {
     FewRing r{STAGES};
-    int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
     for (int i = lo; i < hi; ++i) {
       ok = r.wait_empty(bars, p.status);
       if (!ok) break;
+      const int n = min(Tile::CHUNKS, chunks - c);
+      uint8_t* st = ring + r.s * STAGE;
+      uint64_t* bar = &bars.full[r.s];
+      const int slot = lane < p.T ? plan.slot[d][lane & 7] : 255;
+      const uint32_t meet = __ballot_sync(0xffffffffu, slot != 255);
       if (elect_one()) {
-        const int n = min(Tile::CHUNKS, chunks - c), e = plan.expert[d];
-        const uint2 sl = *reinterpret_cast<const uint2*>(plan.slot[d]);
-        uint8_t* st = ring + r.s * STAGE;
-        uint64_t* bar = &bars.full[r.s];
-        int meet = 0;
-        for (int t = 0; t < p.T; ++t) meet += ((t < 4 ? sl.x : sl.y) >> (t & 3) * 8 & 255u) != 255u;
-        mbar_expect_tx(bar, n * (Tile::BYTES + meet * 128));
-        for (int j = 0; j < n; ++j) few_copy<W>(st + j * Tile::BYTES, bar, &map, p.down, e, tile, c + j, p.H, p.I);
-        for (int t = 0; t < p.T; ++t) {
-          const uint32_t slot = (t < 4 ? sl.x : sl.y) >> (t & 3) * 8 & 255u;
-          if (slot != 255u) bulk_copy_g2s(st + H_OFF + t * H_LD, p.h + (long long)(t * p.top + slot) * p.I + c * 64, n * 128, bar);
-        }
+        mbar_expect_tx(bar, n * (Tile::BYTES + __popc(meet) * 128));
+        Tile::copy(st, bar, &map, p.down, plan.expert[d], n0, c, n, p.H, p.I);
       }
+      __syncwarp();
+      if (slot != 255) bulk_copy_g2s(st + H_OFF + lane * H_LD, p.h + (long long)(lane * p.top + slot) * p.I + c * 64, n * 128, bar);
       __syncwarp();
       r.next();
       c += Tile::CHUNKS;
@@ -455,56 +684,59 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
     }
     if (!ok) r.drain(bars);
   } else {
-    FewRing r{STAGES};
-    int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    const int r0 = warp * 16 + g;
+    float acc[2][4] = {};
+    FewReader<STAGE> r(&bars, ring, STAGES);
+    const uint32_t place = Tile::place(r0, g, q), scales = Tile::scales(r0), hs = H_OFF + g * H_LD + q * 16;
+    uint32_t meets = lo < hi && plan.slot[d][g] != 255 ? ~0u : 0u;     // else what lies in the token's place is left over
+    auto masked = [](const uint4& v, uint32_t m) { return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m); };
+    int turn = 0;
     for (int i = lo; i < hi; ++i) {
-      ok = r.wait_full(bars, p.status, lane);
-      if (!ok) break;
-      const uint8_t* st = ring + r.s * STAGE;
-      const bool mine = plan.slot[d][g] != 255;
-#pragma unroll
-      for (int j = 0; j < Tile::CHUNKS; ++j) {
-        if (j > 0 && c + j >= chunks) break;
-        const uint8_t* hs = st + H_OFF + g * H_LD + j * 128 + q * 16;
-        const uint4 zero = make_uint4(0, 0, 0, 0);
-        const uint4 b[2] = {mine ? *reinterpret_cast<const uint4*>(hs) : zero, mine ? *reinterpret_cast<const uint4*>(hs + 64) : zero};
-        Tile::mma(acc, st + j * Tile::BYTES, r0, r0 + 8, g, q, b);
+      r.release(lane);
+      if (turn == team && ok && (ok = r.wait(p.status))) {
+        const uint32_t x = r.data + hs;
+        uint4 b[2] = {masked(lds128<0>(x), meets), masked(lds128<64>(x), meets)};
+        Tile::mma(acc, r.data + place, r.data + scales, b);
+        if (c + 1 < chunks) {
+          b[0] = masked(lds128<128>(x), meets);
+          b[1] = masked(lds128<192>(x), meets);
+          Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+        }
       }
+      turn = turn + 1 == TEAMS ? 0 : turn + 1;
       r.next();
       c += Tile::CHUNKS;
       if (c < chunks && i + 1 < hi) continue;
       // an expert's part is done: it counts for the tokens that meet it (weights that are not numbers stay with them)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (plan.slot[d][q * 2 + j] != 255) { sum[j] += acc[j]; sum[2 + j] += acc[2 + j]; }
-        acc[j] = acc[2 + j] = 0.f;
+      for (int j = 0; j < 4; ++j) {
+        if (plan.slot[d][q * 2 + (j & 1)] != 255) { sum[0][j] += acc[0][j]; sum[1][j] += acc[1][j]; }
+        acc[0][j] = acc[1][j] = 0.f;
       }
       c = 0;
-      ++d;
+      if (++d < plan.met) meets = plan.slot[d][g] != 255 ? ~0u : 0u;
     }
   }
-  // rows of the tile are dealt out to the cluster's CTAs, a multiple of 16 each
   __syncwarp();
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");        // of the arrival at the start
-  const int rows = 128 / splits;
   if (warp < 8) {
-    const int owner = warp * 16 / rows, l = warp * 16 - owner * rows;
-    const uint32_t at = dsmem_addr(smem_u32(&red[(rank * rows + l + g) * FEW_TOKENS + q * 2]), uint32_t(owner));
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(at + j * 8 * FEW_TOKENS * 4), "f"(sum[j * 2]), "f"(sum[j * 2 + 1]) : "memory");
+    for (int j = 0; j < 4; ++j) {
+      const int o = (r0 + j * 8) * FEW_TOKENS + q * 2, owner = o / per;
+      asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};"
+                   ::"r"(dsmem_addr(smem_u32(&red[(rank * TEAMS + team) * per + o - owner * per]), uint32_t(owner))), "f"(sum[j >> 1][(j & 1) * 2]), "f"(sum[j >> 1][(j & 1) * 2 + 1])
+                   : "memory");
+    }
   }
+  __syncwarp();
   cluster_sync_all();
-  for (int i = threadIdx.x; i < rows * FEW_TOKENS; i += FEW_THREADS) {
-    const int t = i / rows, l = i - t * rows, n = tile * 128 + rank * rows + l;
-    if (t >= p.T || n >= p.H) continue;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    int n, t;
+    const int i = int(threadIdx.x) + k * FEW_THREADS;
+    if (!output(i, n, t)) continue;
     float v = 0.f;
-    for (int s = 0; s < splits; ++s) v += red[(s * rows + l) * FEW_TOKENS + t];
-    if (p.down_b)
-      for (int j = 0; j < p.top; ++j) v += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
-    p.out[(long long)t * p.H + n] = f2bf(v);
+    for (int s = 0; s < splits * TEAMS; ++s) v += red[s * per + i];
+    p.out[(long long)t * p.H + n] = f2bf(fmaf(v, Tile::SCALE, bias[k]));
   }
 }
 
@@ -513,25 +745,24 @@ bool MakeMapBf16(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, 
 
 template <int W>
 static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
-  using Tile = FewTile<W>;
+  using Tile = FewTile<W, 128>;
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
   const int Hp = (p.H + 63) / 64 * 64;
   const size_t fixed = 1024 + sizeof(FewShared) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16 + size_t(p.T) * (Hp + 32) * 2;
-  // Two CTAs an SM where that leaves each a ring of 48 KiB: more warps to expand and multiply; else one with what there is.
-  const int two = fixed + 48 * 1024 <= FEW_SMEM_TWO;
+  // Two CTAs an SM where that leaves each a ring of 32 KiB: more warps to expand and multiply; else one with what there is.
+  const int two = fixed + 32 * 1024 <= FEW_SMEM_TWO;
   const size_t room = two ? FEW_SMEM_TWO : FEW_SMEM_ONE;
-  if (fixed + 2 * STAGE > room) return -5;
-  p.stages = int(min(size_t(FEW_STAGES), (room - fixed) / STAGE));
+  if (fixed + Tile::TEAMS * STAGE > room) return -5;
+  p.stages = Tile::ring(int(room - fixed), STAGE);
   CUtensorMap gate_up = {}, down = {};
-  if (W == FEW_BF16 && (!MakeMapBf16(&gate_up, p.gate_up, p.E * 2 * p.I, p.H, p.H, 128) || !MakeMapBf16(&down, p.down, p.E * p.H, p.I, p.I, 128))) return -2;
+  if (W == FEW_BF16 && (!MakeMapBf16(&gate_up, p.gate_up, p.E * 2 * p.I, p.H, p.H, 128) || !MakeMapBf16(&down, p.down, p.E * p.H, p.I, p.I, FEW_DOWN_ROWS))) return -2;
   static bool configured[OGB_MAX_DEVICES] = {}, configured_down[OGB_MAX_DEVICES] = {};
   if (!set_max_dyn_smem(few_gate_up_kernel<W>, int(FEW_SMEM_ONE), configured) || !set_max_dyn_smem(few_down_kernel<W>, FEW_DOWN_RING + 1024, configured_down)) return -3;
-  static const int pdl = [] { const char* e = getenv("OGB_PDL"); return (e && e[0] == '0') ? 0 : 1; }();
-  cudaLaunchAttribute attr[2];
+  // Both kernels are launched behind the complete kernels in front of them: CTAs that come in as others leave are placed so that some clusters find no room until the
+  // rest is done (8 tokens of 2 of 8 bf16 experts of 14336 in a row: 913 us a layer with programmatic launches, 590 without).
+  cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {FEW_CLUSTER, 1, 1};
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(FEW_THREADS);
   cfg.stream = stream;
@@ -547,15 +778,14 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
   if (!clusters) {
     cfg.dynamicSmemBytes = room;
     if (cudaOccupancyMaxActiveClusters(&clusters, few_gate_up_kernel<W>, &cfg) != cudaSuccess || clusters < 1) return -4;
+    clusters = min(clusters, FEW_MAX_CTAS / FEW_CLUSTER);
     if (tracked) clusters_at[dev][two] = clusters;
   }
   cfg.dynamicSmemBytes = fixed + p.stages * STAGE;
   cfg.gridDim = dim3(unsigned(clusters * FEW_CLUSTER));
-  cfg.numAttrs = pdl ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, few_gate_up_kernel<W>, gate_up, p) != cudaSuccess) return -4;
-  const int tiles = (p.H + 127) / 128;
-  p.splits = FEW_CLUSTER;
-  while (p.splits > 1 && tiles * p.splits > 2 * sm_count) p.splits /= 2;
+  const int tiles = (p.H + FEW_DOWN_ROWS - 1) / FEW_DOWN_ROWS;
+  p.splits = max(1, min(FEW_CLUSTER, 2 * sm_count / tiles));                          // two CTAs an SM
   attr[0].val.clusterDim = {unsigned(p.splits), 1, 1};
   cfg.dynamicSmemBytes = FEW_DOWN_RING + 1024;
   cfg.gridDim = dim3(unsigned(tiles * p.splits));
@@ -567,7 +797,7 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
 using namespace ogb;
 
 OGB_API long long ogb_moe_few_scratch_bytes(int T, int top, int I) {
-  return T < 1 || T > FEW_TOKENS || top < 1 || top > FEW_TOP || I < 1 ? -1 : (long long)sizeof(FewPlan) + (long long)T * top * I * 2;
+  return T < 1 || T > FEW_TOKENS || top < 1 || top > FEW_TOP || I < 1 ? -1 : (long long)sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL + (long long)T * top * I * 2;
 }
 
 OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b,
@@ -579,8 +809,9 @@ OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router,
     return -1;
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,
             static_cast<const __nv_bfloat16*>(gate_up_b), down, static_cast<const __nv_bfloat16*>(down_b), static_cast<__nv_bfloat16*>(out), T, H, I, E, top,
-            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)), 0, 0, status};
-  if ((long long)E * 2 * I > 0x7fffffff || (long long)E * H > 0x7fffffff) return -5;
+            rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<float4*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)),
+            reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL), 0, 0, status};
+  if ((long long)E * 2 * I > 0x7fffffff || (long long)E * H > 0x7fffffff || (long long)min(E, T * top) * I * H > 1LL << 37) return -5;   // (32-bit counts of steps)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, sm_count, s);
   return weights == FEW_FP4_F16 ? LaunchFew<FEW_FP4_F16>(p, sm_count, s) : LaunchFew<FEW_FP4_BF16>(p, sm_count, s);
