@@ -6,7 +6,8 @@
 // 128 x 128 tile needs 36 KB for 256 cycles.  192 tokens, because two accumulators (drained in turns) and two sets of scales then share the 512 columns of tensor
 // memory: 2 x 192 + 2 x (16 + 32).  A tile starts at a multiple of 64 tokens, two columns of scales.
 //
-// Warps of a CTA: 0 copies, 1 issues scale copies and MMAs (of the cluster's first CTA), both as whole warps with one elected lane; 2..5 drain accumulators 32
+// Warps of a CTA: 0 and 6 copy weights and tokens (one warp with both took 680 cycles a stage, more than its MMAs), 1 issues scale copies and MMAs (of the
+// cluster's first CTA), all as whole warps with one elected lane; 2..5 drain accumulators 32
 // tokens at a time through a staging tile that turns a weight row per thread into 16-byte row segments.  Copies of both CTAs are counted on the first CTA's
 // barrier of a stage; a commit frees the stage in both.  All waits are bounded; after a failed one every role leaves its loop, both CTAs meet at the last cluster
 // barrier and return with the status word set.
@@ -34,7 +35,7 @@ struct Fp4PairArgs {
 };
 
 template <int FORM>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(192, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(224, 1)
 linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sw,
                        const __grid_constant__ CUtensorMap map_sx, const Fp4LinearArgs p, const Fp4PairArgs a) {
   using Cfg = Fp4PairCfg<FORM>;
@@ -84,38 +85,29 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   };
   auto fail = [&](int code) { atomicMax(p.status, code); *abort_flag = 1; };
 
-  if (warp == 0) {
-    // ------------------------------------------------------------------ copies: k-blocks of all tiles, back to back
-    bool waited = !p.pdl, ok = true;
+  if (warp == 0 || warp == 6) {
+    // ------------------------------------------------------------------ copies of all tiles' k-blocks, back to back: weights (warp 0) and tokens (warp 6)
+    const bool tokens = warp == 6;
+    bool ok = true;
     int it = 0, s = 0;
     uint32_t ph = 1;
     const int tiles_w = p.w.padded >> 7, tiles_x = p.a.padded >> 7;
     const uint32_t bytes = uint32_t(FP4_W_BYTES + a.bt / 2 * 128 + Cfg::SF + (a.bt > 128 ? 2 : 1) * Cfg::SF);
-    if (p.pdl && !p.early) { pdl_wait(); waited = true; }
+    // the weights may be fetched before the kernel in front has finished, where it writes none; tokens may not
+    if (p.pdl && (tokens || !p.early)) pdl_wait();
     for (int t = first; t < total && ok; t += step) {
       const Tile x = tile_at(t);
-      const int xrow = x.row0 + int(rank) * (x.cols >> 1);
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (it >= S) ok = __all_sync(0xffffffffu, cluster_wait_bounded(&empty[s], ph, abort_flag));
+      int row = tokens ? x.row0 + int(rank) * (x.cols >> 1) : x.n_tile * FP4_TILE, sf = (tokens ? x.row0 >> 7 : x.n_tile) * STEPS;
+      const int row_step = tokens ? p.a.padded : p.w.padded, sf_step = (tokens ? tiles_x : tiles_w) * STEPS;
+      for (int kb = 0; kb < num_kb; ++kb, row += row_step, sf += sf_step) {
+        if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ph, abort_flag));
         if (!ok) { fail(OGB_ERR_WAIT_TMA); break; }
-        uint8_t* st = smem + s * Cfg::STAGE;
-        const uint32_t bar = dsmem_addr(smem_u32(&full[s]), 0);
-        const bool early = !waited;        // the first weights may go out before the kernel in front has finished; tokens may not
-        auto weights = [&]() {
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * bytes);
-          pair_tma_load_2d(st, &map_w, bar, 0, kb * p.w.padded + x.n_tile * FP4_TILE);
-          pair_tma_load_2d(st + Cfg::SFW_OFF, &map_sw, bar, 0, (kb * tiles_w + x.n_tile) * STEPS);
-        };
-        if (early) {
-          if (elect_one()) weights();
-          __syncwarp();
-          pdl_wait();
-          waited = true;
-        }
         if (elect_one()) {
-          if (!early) weights();
-          pair_tma_load_2d(st + Cfg::X_OFF, &map_x, bar, 0, kb * p.a.padded + xrow);
-          pair_tma_load_2d(st + Cfg::SFX_OFF, &map_sx, bar, 0, (kb * tiles_x + (x.row0 >> 7)) * STEPS);
+          uint8_t* st = smem + s * Cfg::STAGE;
+          const uint32_t bar = dsmem_addr(smem_u32(&full[s]), 0);
+          if (!tokens && rank == 0) mbar_expect_tx(&full[s], 2 * bytes);
+          pair_tma_load_2d(st + (tokens ? Cfg::X_OFF : 0), tokens ? &map_x : &map_w, bar, 0, row);
+          pair_tma_load_2d(st + (tokens ? Cfg::SFX_OFF : Cfg::SFW_OFF), tokens ? &map_sx : &map_sw, bar, 0, sf);
         }
         __syncwarp();
         ++it;
@@ -142,7 +134,7 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
         const uint32_t idesc = fp4_idesc(FORM, 2 * FP4_TILE, x.cols, 0);
         const bool wide = a.bt > 128;
         for (int kb = 0; kb < num_kb; ++kb, set ^= 1) {
-          if (!__all_sync(0xffffffffu, cluster_wait_bounded(&full[s], ph, abort_flag))) { fail(OGB_ERR_WAIT_TMA); ok = false; break; }
+          if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag))) { fail(OGB_ERR_WAIT_TMA); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
             const uint32_t base = smem_u32(smem + s * Cfg::STAGE), sf = tmem + Cfg::SF_COL + set * Cfg::SF_SET;
@@ -190,7 +182,7 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
         ub[k] = in && pair && p.bias ? bf2f(p.bias[n0 + seg + 64 + k]) : 0.f;
       }
       // a failed wait is published in a word only these threads write, before the barrier: all 128 take the same branch
-      if (!cluster_wait_bounded(&acc_full[buf], (j >> 1) & 1, abort_flag, 4000000000ull)) { fail(OGB_ERR_WAIT_MMA); *epi_abort = 1; }
+      if (!mbar_wait_bounded(&acc_full[buf], (j >> 1) & 1, abort_flag, 4000000000ull)) { fail(OGB_ERR_WAIT_MMA); *epi_abort = 1; }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (*epi_abort) break;
       tc_fence_after();
@@ -287,7 +279,7 @@ static int LaunchPair(const Fp4LinearArgs& p, int sm_count, cudaStream_t stream)
       !encode_map_2d(&msx, words, p.a.scales, uint64_t(p.a.num_kb) * (p.a.padded >> 7) * steps, 128, 512, steps * wide, 128, plain)) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(2 * min(pairs, a.n_pairs * a.m_tiles)));
-  cfg.blockDim = dim3(192);
+  cfg.blockDim = dim3(224);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
