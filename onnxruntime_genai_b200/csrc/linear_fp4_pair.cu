@@ -23,11 +23,11 @@ template <int FORM>
 struct Fp4PairCfg {
   static constexpr int SF = fp4_sf_bytes(FORM);
   static constexpr int X_OFF = FP4_W_BYTES, SFW_OFF = X_OFF + FP4P_BT / 2 * 128, SFX_OFF = SFW_OFF + SF;
-  static constexpr int STAGE = SFX_OFF + 2 * SF;                       // codes of 128 weight rows and half of the tokens, scales of 128 weight rows and 256 tokens
-  static constexpr int STAGES = 6;
+  static constexpr int BLOCK = SFX_OFF + 2 * SF;                       // a k-block: codes of 128 weight rows and half of the tokens, scales of 128 weight rows and 256 tokens
+  static constexpr int KB = 2, STAGE = KB * BLOCK, STAGES = 3;         // a role's pass over a stage costs some 650 cycles whatever it holds: two k-blocks
   static constexpr int STAGING = STAGES * STAGE, BARS = STAGING + 32 * FP4P_LD * 4, SMEM = BARS + 256 + 1024;
   static constexpr int SF_COL = 2 * FP4P_BT, SF_SET = 64;              // tensor memory: accumulators, then two sets of scales (16 columns of weights, 32 of tokens)
-  static_assert(STAGE % 1024 == 0 && SMEM <= 227 * 1024 && SF_COL + 2 * SF_SET <= 512, "memory");
+  static_assert(BLOCK % 1024 == 0 && SMEM <= 227 * 1024 && SF_COL + 2 * SF_SET <= 512, "memory");
 };
 
 struct Fp4PairArgs {
@@ -99,16 +99,23 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
       const Tile x = tile_at(t);
       int row = tokens ? x.row0 + int(rank) * (x.cols >> 1) : x.n_tile * FP4_TILE, sf = (tokens ? x.row0 >> 7 : x.n_tile) * STEPS;
       const int row_step = tokens ? p.a.padded : p.w.padded, sf_step = (tokens ? tiles_x : tiles_w) * STEPS;
-      for (int kb = 0; kb < num_kb; ++kb, row += row_step, sf += sf_step) {
+      for (int kb = 0; kb < num_kb; kb += Cfg::KB) {
         if (it >= S) ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ph, abort_flag));
         if (!ok) { fail(OGB_ERR_WAIT_TMA); break; }
         if (elect_one()) {
-          uint8_t* st = smem + s * Cfg::STAGE;
+          const int n = min(Cfg::KB, num_kb - kb);
           const uint32_t bar = dsmem_addr(smem_u32(&full[s]), 0);
-          if (!tokens && rank == 0) mbar_expect_tx(&full[s], 2 * bytes);
-          pair_tma_load_2d(st + (tokens ? Cfg::X_OFF : 0), tokens ? &map_x : &map_w, bar, 0, row);
-          pair_tma_load_2d(st + (tokens ? Cfg::SFX_OFF : Cfg::SFW_OFF), tokens ? &map_sx : &map_sw, bar, 0, sf);
+          if (!tokens && rank == 0) mbar_expect_tx(&full[s], 2 * n * bytes);
+#pragma unroll
+          for (int h = 0; h < Cfg::KB; ++h) {
+            if (h >= n) break;
+            uint8_t* st = smem + s * Cfg::STAGE + h * Cfg::BLOCK;
+            pair_tma_load_2d(st + (tokens ? Cfg::X_OFF : 0), tokens ? &map_x : &map_w, bar, 0, row + h * row_step);
+            pair_tma_load_2d(st + (tokens ? Cfg::SFX_OFF : Cfg::SFW_OFF), tokens ? &map_sx : &map_sw, bar, 0, sf + h * sf_step);
+          }
         }
+        row += Cfg::KB * row_step;
+        sf += Cfg::KB * sf_step;
         __syncwarp();
         ++it;
         if (++s == S) { s = 0; ph ^= 1; }
@@ -121,7 +128,7 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   } else if (warp == 1) {
     if (rank == 0) {
       // ------------------------------------------------------------------ MMAs of the pair: the two accumulators in turns
-      int s = 0, j = 0, set = 0;
+      int s = 0, j = 0;
       uint32_t ph = 0;
       bool ok = true;
       for (int t = first; t < total && ok; t += step, ++j) {
@@ -133,27 +140,32 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
         const uint32_t acc = tmem + uint32_t(buf * FP4P_BT), off = uint32_t(x.row0 & 127) >> 5;      // the tile's first column in a step's scales
         const uint32_t idesc = fp4_idesc(FORM, 2 * FP4_TILE, x.cols, 0);
         const bool wide = a.bt > 128;
-        for (int kb = 0; kb < num_kb; ++kb, set ^= 1) {
+        for (int kb = 0; kb < num_kb; kb += Cfg::KB) {
           if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full[s], ph, abort_flag))) { fail(OGB_ERR_WAIT_TMA); ok = false; break; }
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t base = smem_u32(smem + s * Cfg::STAGE), sf = tmem + Cfg::SF_COL + set * Cfg::SF_SET;
-            const uint64_t dw = umma_desc_sw128(base), dx = umma_desc_sw128(base + Cfg::X_OFF);
-            const uint64_t dsw = fp4_scale_desc(base + Cfg::SFW_OFF), dsx = fp4_scale_desc(base + Cfg::SFX_OFF);
+            const int n = min(Cfg::KB, num_kb - kb);
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-              fp4_copy_scales<2>(sf + k * 4, dsw + k * (FP4_SCALE_STEP >> 4));
-              fp4_copy_scales<2>(sf + 16 + k * 8, dsx + k * (FP4_SCALE_STEP >> 4));
-              if (wide) fp4_copy_scales<2>(sf + 16 + k * 8 + 4, dsx + (STEPS + k) * (FP4_SCALE_STEP >> 4));
-            }
+            for (int h = 0; h < Cfg::KB; ++h) {
+              if (h >= n) break;
+              const uint32_t base = smem_u32(smem + s * Cfg::STAGE + h * Cfg::BLOCK), sf = tmem + Cfg::SF_COL + h * Cfg::SF_SET;
+              const uint64_t dw = umma_desc_sw128(base), dx = umma_desc_sw128(base + Cfg::X_OFF);
+              const uint64_t dsw = fp4_scale_desc(base + Cfg::SFW_OFF), dsx = fp4_scale_desc(base + Cfg::SFX_OFF);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int st = FORM == FP4_NV ? k : k >> 1;
-              const uint32_t id = FORM == FP4_NV ? 0u : uint32_t(k & 1) * 2u;
-              fp4_mma<2, FORM>(acc, dw + k * 2, dx + k * 2, idesc | id << 4 | id << 29, sf + st * 4, sf + 16 + st * 8 + off, kb > 0 || k > 0 ? 1u : 0u);
+              for (int k = 0; k < STEPS; ++k) {
+                fp4_copy_scales<2>(sf + k * 4, dsw + k * (FP4_SCALE_STEP >> 4));
+                fp4_copy_scales<2>(sf + 16 + k * 8, dsx + k * (FP4_SCALE_STEP >> 4));
+                if (wide) fp4_copy_scales<2>(sf + 16 + k * 8 + 4, dsx + (STEPS + k) * (FP4_SCALE_STEP >> 4));
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int st = FORM == FP4_NV ? k : k >> 1;
+                const uint32_t id = FORM == FP4_NV ? 0u : uint32_t(k & 1) * 2u;
+                fp4_mma<2, FORM>(acc, dw + k * 2, dx + k * 2, idesc | id << 4 | id << 29, sf + st * 4, sf + 16 + st * 8 + off, kb > 0 || h > 0 || k > 0 ? 1u : 0u);
+              }
             }
             pair_commit(&empty[s]);
-            if (kb == num_kb - 1) pair_commit(&acc_full[buf]);
+            if (kb + Cfg::KB >= num_kb) pair_commit(&acc_full[buf]);
           }
           __syncwarp();
           if (++s == S) { s = 0; ph ^= 1; }
