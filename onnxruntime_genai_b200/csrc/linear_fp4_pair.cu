@@ -6,9 +6,8 @@
 // 128 x 128 tile needs 36 KB for 256 cycles.  192 tokens, because two accumulators (drained in turns) and two sets of scales then share the 512 columns of tensor
 // memory: 2 x 192 + 2 x (16 + 32).  A tile starts at a multiple of 64 tokens, two columns of scales.
 //
-// Warps of a CTA: 0 and 6 copy weights and tokens (one warp with both took 680 cycles a stage, more than its MMAs), 1 issues scale copies and MMAs (of the
-// cluster's first CTA), all as whole warps with one elected lane; 2..5 drain accumulators 32
-// tokens at a time through a staging tile that turns a weight row per thread into 16-byte row segments.  Copies of both CTAs are counted on the first CTA's
+// Warps of a CTA: 0 and 2 copy weights and tokens, 1 issues scale copies and MMAs (of the cluster's first CTA), all as whole warps with one elected lane; 3..10 drain
+// accumulators, two teams 16 tokens at a time through staging tiles that turn a weight row per thread into 16-byte row segments.  Copies of both CTAs are counted on the first CTA's
 // barrier of a stage; a commit frees the stage in both.  All waits are bounded; after a failed one every role leaves its loop, both CTAs meet at the last cluster
 // barrier and return with the status word set.
 #include "kernels.h"
@@ -35,7 +34,7 @@ struct Fp4PairArgs {
 };
 
 template <int FORM>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(224, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(352, 1)
 linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_sw,
                        const __grid_constant__ CUtensorMap map_sx, const Fp4LinearArgs p, const Fp4PairArgs a) {
   using Cfg = Fp4PairCfg<FORM>;
@@ -49,16 +48,16 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   uint64_t* acc_empty = acc_full + 2;                                  // [2] drain of both CTAs -> MMA (first CTA's)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile int* epi_abort = reinterpret_cast<volatile int*>(tmem_slot + 2);
+  volatile int* epi_abort = reinterpret_cast<volatile int*>(tmem_slot + 2);     // [team]
 
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1, num_kb = p.w.num_kb, total = a.m_tiles * a.n_pairs;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
-    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 8); }
+    for (int b = 0; b < 2; ++b) { mbar_init(&acc_full[b], 1); mbar_init(&acc_empty[b], 16); }
     *abort_flag = 0;
-    *epi_abort = 0;
+    epi_abort[0] = epi_abort[1] = 0;
     mbar_fence_init();
     tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
@@ -85,9 +84,9 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
   };
   auto fail = [&](int code) { atomicMax(p.status, code); *abort_flag = 1; };
 
-  if (warp == 0 || warp == 6) {
-    // ------------------------------------------------------------------ copies of all tiles' k-blocks, back to back: weights (warp 0) and tokens (warp 6)
-    const bool tokens = warp == 6;
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------------------ copies of all tiles' k-blocks, back to back: weights (warp 0) and tokens (warp 2)
+    const bool tokens = warp == 2;
     bool ok = true;
     int it = 0, s = 0;
     uint32_t ph = 1;
@@ -173,9 +172,11 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
       }
     }
   } else {
-    // -------------------------------------------------------------------- drain: warps 2..5
-    const int et = int(threadIdx.x) - 64, quarter = warp & 3, row = quarter * 32 + lane;
+    // -------------------------------------------------------------------- drain: two teams of four warps take turns at 16 tokens
+    const int et = (int(threadIdx.x) - 96) & 127, team = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const bool pair = p.pair != 0;
+    float* mine = staging + team * 16 * FP4P_LD;
+    auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + team) : "memory"); };
     // the eight columns of a token row that this thread finishes: plain, of its own warp's rows; paired, of the 64 gate rows
     const int seg = pair ? (et & 7) * 8 : quarter * 32 + (lane & 3) * 8, tok = pair ? et >> 3 : lane >> 2;
     if (p.pdl) pdl_wait();
@@ -193,57 +194,45 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
         us[k] = in && pair ? p.w.row_scale[n0 + seg + 64 + k] : 0.f;
         ub[k] = in && pair && p.bias ? bf2f(p.bias[n0 + seg + 64 + k]) : 0.f;
       }
-      // a failed wait is published in a word only these threads write, before the barrier: all 128 take the same branch
-      if (!mbar_wait_bounded(&acc_full[buf], (j >> 1) & 1, abort_flag, 4000000000ull)) { fail(OGB_ERR_WAIT_MMA); *epi_abort = 1; }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (*epi_abort) break;
+      // a failed wait is published in a word, before the barrier: the team takes the same branch
+      if (!mbar_wait_bounded(&acc_full[buf], (j >> 1) & 1, abort_flag, 4000000000ull)) { fail(OGB_ERR_WAIT_MMA); epi_abort[team] = 1; }
+      __syncwarp();
+      meet();
+      if (epi_abort[team]) break;
       tc_fence_after();
       const uint32_t taddr = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(buf * FP4P_BT);
-      for (int c0 = 0; c0 < rows; c0 += 32) {
-        uint32_t r0[16], r1[16];
+      for (int c0 = team * 16; c0 < rows; c0 += 32) {
+        uint32_t r[16];
         __syncwarp();
-        tmem_ld16(taddr + c0, r0);
-        tmem_ld16(taddr + c0 + 16, r1);
+        tmem_ld16(taddr + c0, r);
         tmem_ld_wait();
 #pragma unroll
-        for (int q = 0; q < 16; ++q) {
-          staging[q * FP4P_LD + row] = __uint_as_float(r0[q]);
-          staging[(q + 16) * FP4P_LD + row] = __uint_as_float(r1[q]);
-        }
+        for (int q = 0; q < 16; ++q) mine[q * FP4P_LD + row] = __uint_as_float(r[q]);
         // all values of the chunk are read before the first store: a store through a generic pointer would order the reads behind it
         if (pair) {
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          float4 g[2][2], h[2][2];
+          meet();
+          const float4* src = reinterpret_cast<const float4*>(mine + tok * FP4P_LD + seg);
+          const float4 g0 = src[0], g1 = src[1], h0 = src[16], h1 = src[17];
+          const float sc = p.a.row_scale[x.row0 + c0 + tok];                      // (padded to whole tiles)
+          meet();
+          float v[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+          const float u[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = silu(fmaf(v[q], sc * ws[q], wb[q])) * fmaf(u[q], sc * us[q], ub[q]);
+          if (c0 + tok < rows && col < p.n_out) fp4_store8(p, x.row0 + c0 + tok, col, v);
+        } else {
+          __syncwarp();
+          float4 g[2][2];
           float sc[2];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
-            const float4* src = reinterpret_cast<const float4*>(staging + (tok + k * 16) * FP4P_LD + seg);
-            g[k][0] = src[0]; g[k][1] = src[1]; h[k][0] = src[16]; h[k][1] = src[17];
-            sc[k] = p.a.row_scale[x.row0 + c0 + tok + k * 16];                 // (padded to whole tiles)
-          }
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int m = c0 + tok + k * 16;
-            float v[8] = {g[k][0].x, g[k][0].y, g[k][0].z, g[k][0].w, g[k][1].x, g[k][1].y, g[k][1].z, g[k][1].w};
-            const float u[8] = {h[k][0].x, h[k][0].y, h[k][0].z, h[k][0].w, h[k][1].x, h[k][1].y, h[k][1].z, h[k][1].w};
-#pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = silu(fmaf(v[q], sc[k] * ws[q], wb[q])) * fmaf(u[q], sc[k] * us[q], ub[q]);
-            if (m < rows && col < p.n_out) fp4_store8(p, x.row0 + m, col, v);
-          }
-        } else {
-          __syncwarp();
-          float4 g[4][2];
-          float sc[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float4* src = reinterpret_cast<const float4*>(staging + (tok + k * 8) * FP4P_LD + seg);
+            const float4* src = reinterpret_cast<const float4*>(mine + (tok + k * 8) * FP4P_LD + seg);
             g[k][0] = src[0]; g[k][1] = src[1];
             sc[k] = p.a.row_scale[x.row0 + c0 + tok + k * 8];
           }
           __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2; ++k) {
             const int m = c0 + tok + k * 8;
             float v[8] = {g[k][0].x, g[k][0].y, g[k][0].z, g[k][0].w, g[k][1].x, g[k][1].y, g[k][1].z, g[k][1].w};
 #pragma unroll
@@ -291,7 +280,7 @@ static int LaunchPair(const Fp4LinearArgs& p, int sm_count, cudaStream_t stream)
       !encode_map_2d(&msx, words, p.a.scales, uint64_t(p.a.num_kb) * (p.a.padded >> 7) * steps, 128, 512, steps * wide, 128, plain)) return -2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(2 * min(pairs, a.n_pairs * a.m_tiles)));
-  cfg.blockDim = dim3(224);
+  cfg.blockDim = dim3(352);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr;
