@@ -4,8 +4,8 @@
 // Both operands go to the block-scaled tensor-core product (`tcgen05.mma.kind::mxf4nvf4.block_scale`) as they are: codes from shared memory, block
 // scales from tensor memory, fp32 accumulators.  Weights are the M operand (128 rows a CTA), tokens the N operand.
 //
-// Few tokens (linear_fp4_kernel): bound by the weights' bytes.  A CTA holds one tile of 128 weight rows x BT tokens of a part of the k-blocks; the parts of a
-// tile form a cluster that sums its accumulators through distributed shared memory, always in the same order.
+// Up to 64 tokens (linear_fp4_kernel): bound by the weights' bytes.  A CTA holds one tile of 128 weight rows x BT tokens of a part of the k-blocks; the parts of a
+// tile form a cluster that sums its accumulators through distributed shared memory, always in the same order.  More tokens: linear_fp4_pair.cu.
 #include "kernels.h"
 #include "linear_fp4.cuh"
 #include "packed_weights.cuh"
@@ -23,8 +23,8 @@ struct Fp4Cfg {
   static constexpr int SUMS = (BT + 8) * FP4_TILE * 4;
   static constexpr int STAGES = (110 * 1024 - (APART ? SUMS : 0)) / STAGE;         // two CTAs per SM
   static constexpr int SF_COL = BT < 32 ? 32 : BT;                                // first tensor-memory column of the scales: two sets of 16 + 16
-  static constexpr int COLS = SF_COL + 64 <= 128 ? 128 : 256;
-  static_assert(STAGE % 1024 == 0 && STAGES >= 2, "stages");
+  static constexpr int COLS = 128;
+  static_assert(STAGE % 1024 == 0 && STAGES >= 2 && SF_COL + 64 <= COLS, "stages, tensor memory");
   static constexpr int smem(int stages) {
     const int ring = stages * STAGE;
     return (APART ? ring + SUMS : ring > SUMS ? ring : SUMS) + 1024 + 256;
@@ -44,7 +44,7 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int n_tile = blockIdx.x, row0 = blockIdx.y * BT, rows = min(BT, p.a.rows - row0);
+  const int n_tile = blockIdx.x, rows = p.a.rows;           // at most BT
   const int kb0 = blockIdx.z * p.kb_per_split, num = min(p.kb_per_split, p.w.num_kb - kb0);       // at least one
   auto fail = [&](int code) { atomicMax(p.status, code); *abort_flag = 1; };
 
@@ -66,8 +66,8 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
     // ---------------------------------------------------------------- copies
     const uint8_t* w = p.w.codes + (long long)n_tile * FP4_W_BYTES;
     const uint8_t* sw = p.w.scales + (long long)n_tile * Cfg::SF;
-    const uint8_t* x = p.a.codes + (long long)row0 * 128;
-    const uint8_t* sx = p.a.scales + (long long)(row0 >> 7) * Cfg::SF;
+    const uint8_t* x = p.a.codes;
+    const uint8_t* sx = p.a.scales;
     const long long w_step = (long long)p.w.padded * 128, x_step = (long long)p.a.padded * 128;
     const long long sw_step = (long long)(p.w.padded >> 7) * Cfg::SF, sx_step = (long long)(p.a.padded >> 7) * Cfg::SF;
     auto weights = [&](int i, int s) {
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
     const int col = n_tile * (p.pair ? 64 : 128) + seg;
     if (col < p.n_out) {
       for (int m = first + (p.pair ? et >> 3 : et >> 4); m < last; m += 128 / segs) {
-        const float scale = p.a.row_scale[row0 + m];
+        const float scale = p.a.row_scale[m];
         float v[8], u[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = u[j] = 0.f;
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = silu(v[j]) * fmaf(u[j], scale * us[j], ub[j]);
         }
-        fp4_store8(p, row0 + m, col, v);
+        fp4_store8(p, m, col, v);
       }
     }
   }
@@ -224,7 +224,7 @@ static int LaunchFew(Fp4LinearArgs p, int splits, cudaStream_t stream) {
   p.splits = splits = (p.w.num_kb + p.kb_per_split - 1) / p.kb_per_split;
   p.stages = min(Cfg::STAGES, p.kb_per_split);       // no more shared memory than the CTA has k-blocks: the next kernel's CTAs find room
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(p.w.padded / FP4_TILE), unsigned((p.a.rows + BT - 1) / BT), unsigned(splits));
+  cfg.gridDim = dim3(unsigned(p.w.padded / FP4_TILE), 1u, unsigned(splits));
   cfg.blockDim = dim3(192);
   cfg.dynamicSmemBytes = Cfg::smem(p.stages);
   cfg.stream = stream;
@@ -246,14 +246,15 @@ static int LaunchFew(Fp4LinearArgs p, int splits, cudaStream_t stream) {
 
 template <int FORM>
 static int LaunchLinear(const Fp4LinearArgs& p, int sm_count, cudaStream_t stream) {
-  const int T = p.a.rows, bt = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-  if (T > 128) return LaunchPairLinearFp4(p, FORM, sm_count, stream);
-  const int tiles = p.w.padded / FP4_TILE * ((T + bt - 1) / bt);
+  const int T = p.a.rows, bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
+  // (65 / 128 tokens, us here against pairs of SMs: 6144 x 4096 14.5 / 20.4 against 7.1 / 7.5, 28672 x 4096 14.5 / 17.6 against 12.2 / 13.7, 4096 x 14336 11.8 / 16.1
+  // against 14.5 / 14.7)
+  if (T > 64) return LaunchPairLinearFp4(p, FORM, sm_count, stream);
+  const int tiles = p.w.padded / FP4_TILE;
   const int splits = max(1, min(min(8, p.w.num_kb), 2 * sm_count / tiles));
   if (bt == 16) return LaunchFew<16, FORM>(p, splits, stream);
   if (bt == 32) return LaunchFew<32, FORM>(p, splits, stream);
-  if (bt == 64) return LaunchFew<64, FORM>(p, splits, stream);
-  return LaunchFew<128, FORM>(p, splits, stream);
+  return LaunchFew<64, FORM>(p, splits, stream);
 }
 
 }  // namespace ogb
@@ -265,7 +266,6 @@ OGB_API int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_dat
   if (!w_data || T < 0 || (T > 0 && (!a_data || !out)) || N <= 0 || K <= 0 || (form != FP4_NV && form != FP4_MX) || K % fp4_block(form)) return -1;
   if ((reinterpret_cast<uintptr_t>(a_data) | reinterpret_cast<uintptr_t>(w_data)) & 15) return -1;
   if (pair && (N % 128 || residual)) return -1;
-  if (T > 65535 * 128) return -5;
   if (T == 0) return 0;
   if (x) {
     const int rc = ogb_quantize_fp4(x, ldx, x_fp32, T, K, form, a_data, stream);

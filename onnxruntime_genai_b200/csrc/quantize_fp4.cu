@@ -65,6 +65,15 @@ template <> struct Raw8<__nv_bfloat16> {
     }
   }
   __device__ __forceinline__ void zero() { q = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t largest() const {        // bits of the largest magnitude, as fp32
+    const uint32_t m = 0x7fff7fffu, a = max2(max2(q.x & m, q.y & m), max2(q.z & m, q.w & m));
+    return max(a & 0xffff0000u, a << 16);
+  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -78,25 +87,34 @@ template <> struct Raw8<float> {
     else { a = make_float4(p[0], p[1], p[2], p[3]); b = make_float4(p[4], p[5], p[6], p[7]); }
   }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ uint32_t largest() const {
+    float v[8];
+    get(v);
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+    return m;
+  }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
 };
 
 // A warp turns a row's k-blocks of 256, eight elements a lane: a block of 16 (32) belongs to two (four) lanes, the codes of a k-block go out as one
-// line of 128 bytes.  `wpr` warps share a row (a power of two, as many as it has k-blocks up to 16) and meet once, at the row's largest value; up to
-// QUANT_HELD k-blocks a warp stay in registers between the two passes, later ones are read again.
-constexpr int QUANT_HELD = 4;
-template <typename T, int FORM, bool VEC>
-__global__ void __launch_bounds__(512) quantize_fp4_kernel(const T* __restrict__ x, long long ldx, int K, int wpr, Fp4View out) {
+// line of 128 bytes.  `wpr` warps share a row (a power of two up to THREADS / 32) and meet once, at the row's largest value; up to
+// HELD k-blocks a warp stay in registers between the two passes, later ones are read again.
+// Bound by bandwidth with many rows, which takes many bytes in flight: 256 threads with eight pieces each, three CTAs an SM (512 threads with four, two an SM: 4096 x
+// 14336 in 65 us); by latency with few, where twice the warps share a row.
+template <typename T, int FORM, bool VEC, int HELD, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_kernel(const T* __restrict__ x, long long ldx, int K, int wpr, Fp4View out) {
   __shared__ uint32_t s_top[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, first = warp & (wpr - 1);
-  const int row = blockIdx.x * (int(blockDim.x >> 5) / wpr) + warp / wpr;
+  const int row = blockIdx.x * (THREADS / 32 / wpr) + warp / wpr;
   const bool here = row < out.rows;
   const T* src = x + (long long)(here ? row : 0) * ldx;
   pdl_wait();
   pdl_launch_dependents();     // after the wait: whoever starts now may read what the kernels before this one wrote (linear_fp4.cu does)
-  Raw8<T> held[QUANT_HELD];
+  Raw8<T> held[HELD];
   uint32_t top = 0;
   auto fetch = [&](int kb) {
     Raw8<T> r;
@@ -104,17 +122,11 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const T* __restrict__
     if (here && k < K) r.template load<VEC>(src + k); else r.zero();        // K is a multiple of 16: all eight or none
     return r;
   };
-  auto largest = [&](const Raw8<T>& r) {
-    float v[8];
-    r.get(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(v[i]));
-  };
+  for (int i = 0; i < HELD; ++i) held[i] = fetch(first + i * wpr);
 #pragma unroll
-  for (int i = 0; i < QUANT_HELD; ++i) held[i] = fetch(first + i * wpr);
-#pragma unroll
-  for (int i = 0; i < QUANT_HELD; ++i) largest(held[i]);
-  for (int kb = first + QUANT_HELD * wpr; kb < out.num_kb; kb += wpr) largest(fetch(kb));
+  for (int i = 0; i < HELD; ++i) top = max(top, held[i].largest());
+  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) top = max(top, fetch(kb).largest());
   top = __reduce_max_sync(0xffffffffu, top);
   if (wpr > 1) {
     if (lane == 0) s_top[warp] = top;
@@ -124,29 +136,24 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const T* __restrict__
   if (!here) return;
   const bool bad = top >= 0x7f800000u;
   const int re = FORM == FP4_NV ? row_exponent(top) : 0;
-  if (first == 0 && lane == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : pow2(re);
-  const float over = pow2(-re);
+  const float s = pow2(re), over = pow2(-re);
+  if (first == 0 && lane == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
 
   auto emit = [&](const Raw8<T>& r, int kb) {
     float v[8];
-    uint32_t m = 0;
+    uint32_t m = r.largest();
     r.get(v);
-    if (FORM == FP4_NV) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= over;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     uint32_t code;
     if (FORM == FP4_NV) {
-      code = bad ? 0u : e4m3_of(__fdiv_rn(__uint_as_float(m), 6.f));
-      const float sc = fp4_scale_nv(code), inv = code ? __frcp_rn(sc) : 0.f;
-      // v / sc: a product with the rounded reciprocal and one correction by the exact remainder, so that a quotient that is a tie comes out as that tie
+      code = bad ? 0u : e4m3_of(__fdiv_rn(__uint_as_float(m) * over, 6.f));
+      // x / (scale s): a product with the rounded reciprocal and one correction by the exact remainder, so that a quotient that is a tie comes out as that tie (the
+      // powers of two of s change no rounding)
+      const float sc = fp4_scale_nv(code), by = sc * s, inv = code ? __frcp_rn(sc) * over : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float q = v[i] * inv;
-        v[i] = fmaf(fmaf(-q, sc, v[i]), inv, q);
+        v[i] = fmaf(fmaf(-q, by, v[i]), inv, q);
       }
     } else {
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -166,9 +173,9 @@ __global__ void __launch_bounds__(512) quantize_fp4_kernel(const T* __restrict__
       *reinterpret_cast<uint32_t*>(out.scales + fp4_scale_at(out, FORM, kb, row, lane / (4 * PER), 0)) = code | c1 << 8 | c2 << 16 | c3 << 24;
   };
 #pragma unroll
-  for (int i = 0; i < QUANT_HELD; ++i)
+  for (int i = 0; i < HELD; ++i)
     if (first + i * wpr < out.num_kb) emit(held[i], first + i * wpr);
-  for (int kb = first + QUANT_HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb), kb);
+  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb), kb);
 }
 
 // A warp reads four rows of a k-block (512 bytes of codes), eight elements a lane and row.
@@ -206,16 +213,23 @@ __global__ void __launch_bounds__(256) dequantize_fp4_kernel(Fp4View m, int K, T
   }
 }
 
+template <typename T, int FORM, bool VEC>
+static bool LaunchQuantize(const T* x, long long ldx, int K, const Fp4View& v, cudaStream_t s) {
+  const bool few = v.rows <= 296;                   // two CTAs of 512 threads an SM
+  constexpr int HELD = sizeof(T) == 2 ? 8 : 4;
+  const int warps = few ? 16 : 8, each = few ? 1 : HELD;      // k-blocks that a warp is to have of a row, where it has so many
+  int wpr = 1;
+  while (wpr * each < v.num_kb && wpr < warps) wpr *= 2;
+  const int rows_per_cta = warps / wpr;
+  const dim3 grid(unsigned((v.rows + rows_per_cta - 1) / rows_per_cta)), block(unsigned(warps * 32));
+  return few ? launch_pdl(quantize_fp4_kernel<T, FORM, VEC, 4, 512>, grid, block, 0, s, x, ldx, K, wpr, v)
+             : launch_pdl(quantize_fp4_kernel<T, FORM, VEC, HELD, 256>, grid, block, 0, s, x, ldx, K, wpr, v);
+}
 template <typename T, int FORM>
 static bool LaunchQuantize(const void* x, long long ldx, int K, const Fp4View& v, cudaStream_t s) {
-  int wpr = 1;
-  while (wpr < v.num_kb && wpr < 16) wpr *= 2;
-  const int warps = wpr == 16 ? 16 : 8, rows_per_cta = warps / wpr;
-  const dim3 grid(unsigned((v.rows + rows_per_cta - 1) / rows_per_cta)), block(unsigned(warps * 32));
   const T* p = static_cast<const T*>(x);
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * (long long)sizeof(T))) & 15) == 0;
-  return vec ? launch_pdl(quantize_fp4_kernel<T, FORM, true>, grid, block, 0, s, p, ldx, K, wpr, v)
-             : launch_pdl(quantize_fp4_kernel<T, FORM, false>, grid, block, 0, s, p, ldx, K, wpr, v);
+  return vec ? LaunchQuantize<T, FORM, true>(p, ldx, K, v, s) : LaunchQuantize<T, FORM, false>(p, ldx, K, v, s);
 }
 template <typename T>
 static bool LaunchDequantize(const Fp4View& v, int K, int form, void* out, long long ldo, cudaStream_t s) {
