@@ -139,17 +139,24 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
   const float s = pow2(re), over = pow2(-re);
   if (first == 0 && lane == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
 
-  auto emit = [&](const Raw8<T>& r, int kb) {
+  constexpr int PER = FORM == FP4_NV ? 2 : 4;                              // lanes of a block; four blocks' scales are one word
+  uint8_t* codes_to = out.codes + fp4_code_at(out, first, row, lane >> 2) + (lane & 3) * 4;
+  uint8_t* scales_to = out.scales + fp4_scale_at(out, FORM, first, row, lane / (4 * PER), 0);
+  const long long codes_step = (long long)wpr * out.padded * 128, scales_step = (long long)wpr * (out.padded >> 7) * (fp4_steps(FORM) * FP4_SCALE_STEP);
+  auto emit = [&](const Raw8<T>& r) {
     float v[8];
     uint32_t m = r.largest();
     r.get(v);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     uint32_t code;
     if (FORM == FP4_NV) {
-      code = bad ? 0u : e4m3_of(__fdiv_rn(__uint_as_float(m) * over, 6.f));
-      // x / (scale s): a product with the rounded reciprocal and one correction by the exact remainder, so that a quotient that is a tie comes out as that tie (the
-      // powers of two of s change no rounding)
-      const float sc = fp4_scale_nv(code), by = sc * s, inv = code ? __frcp_rn(sc) * over : 0.f;
+      // Quotients are products with the rounded reciprocal and one correction by the exact remainder, so that one that is a tie comes out as that tie.  The powers
+      // of two of the row's scale change no rounding.
+      constexpr float sixth = 1.f / 6.f;
+      const float t = __uint_as_float(m) * over, h = t * sixth;
+      code = bad ? 0u : e4m3_of(fmaf(fmaf(-h, 6.f, t), sixth, h));
+      const float sc = fp4_scale_nv(code), by = sc * s, near = __fdividef(1.f, sc);
+      const float inv = code ? fmaf(fmaf(-sc, near, 1.f), near, near) * over : 0.f;      // (a Newton step makes the approximate reciprocal the nearest one)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float q = v[i] * inv;
@@ -161,21 +168,20 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
       if (m < 0x00800000u) e = m ? -118 - __clz(m) : -127;                 // below the normal numbers: m 2^-149
       e = max(e - 2, -127);
       code = bad ? 0u : uint32_t(e + 127);
-      const float inv = pow2(-e);
+      const float inv = __uint_as_float(uint32_t(127 - e) << 23);          // (of a row that is not numbers: whatever)
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= inv;
     }
-    const uint32_t codes = bad ? 0u : e2m1x8(v);
-    *reinterpret_cast<uint32_t*>(out.codes + fp4_code_at(out, kb, row, lane >> 2) + (lane & 3) * 4) = codes;
-    constexpr int PER = FORM == FP4_NV ? 2 : 4;                              // lanes of a block; four blocks' scales are one word
+    *reinterpret_cast<uint32_t*>(codes_to) = bad ? 0u : e2m1x8(v);
     const uint32_t c1 = __shfl_down_sync(0xffffffffu, code, PER), c2 = __shfl_down_sync(0xffffffffu, code, 2 * PER), c3 = __shfl_down_sync(0xffffffffu, code, 3 * PER);
-    if (lane % (4 * PER) == 0)
-      *reinterpret_cast<uint32_t*>(out.scales + fp4_scale_at(out, FORM, kb, row, lane / (4 * PER), 0)) = code | c1 << 8 | c2 << 16 | c3 << 24;
+    if (lane % (4 * PER) == 0) *reinterpret_cast<uint32_t*>(scales_to) = code | c1 << 8 | c2 << 16 | c3 << 24;
+    codes_to += codes_step;
+    scales_to += scales_step;
   };
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
-    if (first + i * wpr < out.num_kb) emit(held[i], first + i * wpr);
-  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb), kb);
+    if (first + i * wpr < out.num_kb) emit(held[i]);
+  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb));
 }
 
 // A warp reads four rows of a k-block (512 bytes of codes), eight elements a lane and row.
