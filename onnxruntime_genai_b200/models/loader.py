@@ -305,6 +305,27 @@ def _q4_weight(g: GraphView, nodes, device, interleave: bool = False):
     return W4Weight.from_quantized(q, s, z, device, interleaved=interleave)
 
 
+def _is_fp4(nodes) -> bool:
+    return all(n is not None and n.op_type == "MatMulBlockQuantizedFp4Weight" for n in nodes)
+
+
+def _fp4_weight(g: GraphView, nodes, device, interleave: bool = False):
+    """One Fp4Matrix from one or more MatMulBlockQuantizedFp4Weight nodes stacked along N: the checkpoint's codes and block scales as they are, each
+    node's global scale as the scale of its rows."""
+    from ..ops.fp4_matrix import Fp4Matrix
+    codes, scales, rows = [], [], []
+    for n in nodes:
+        c = g.tensor(n.inputs[1]).to(device)
+        codes.append(c.view(torch.uint8))
+        scales.append(g.tensor(n.inputs[2]).to(device).view(torch.uint8).reshape(c.shape[0], -1))
+        rows.append(g.tensor(n.inputs[3]).float().to(device).reshape(1).expand(c.shape[0]))
+    parts = [torch.cat(t, 0) for t in (codes, scales, rows)]
+    if interleave:
+        from ..ops import interleave_gate_up
+        parts = [interleave_gate_up(t) for t in parts]
+    return Fp4Matrix.from_codes(*parts, interleaved=interleave)
+
+
 def _vec(g: GraphView, name: str, dtype, device, sl: Optional[slice] = None) -> Optional[torch.Tensor]:
     if not g.has_init(name):
         return None
@@ -328,6 +349,8 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
     tpn, tpr = model.tp.size, model.tp.rank
     # int4 MatMulNBits weights stay int4 (dequant GEMM) on a single GPU; tensor-parallel shards are dequantised to bf16
     keep_q4 = tpn == 1 and os.environ.get("OGB_DEQUANT_INT4_AT_LOAD", "0") != "1"
+    # NVFP4 weights are expanded, unless it is asked for that they stay packed: their products then quantise the rows to 4 bits too
+    keep_fp4 = tpn == 1 and os.environ.get("OGB_FP4_LINEAR", "0") == "1"
     if arch.num_heads % tpn or (arch.num_kv_heads % tpn and tpn % arch.num_kv_heads):
         raise ValueError(f"tensor parallel degree {tpn} does not divide the attention heads")
     if arch.num_kv_heads < tpn:
@@ -337,6 +360,12 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
     q_rows = slice(tpr * hq_l * D, (tpr + 1) * hq_l * D)
     k_rows = slice(Hq * D + tpr * hkv_l * D, Hq * D + (tpr + 1) * hkv_l * D)
     v_rows = slice(Hq * D + Hkv * D + tpr * hkv_l * D, Hq * D + Hkv * D + (tpr + 1) * hkv_l * D)
+
+    def packed_weight(node, interleave=False):
+        """A weight that stays as the checkpoint packs it, or None."""
+        if keep_q4 and _is_q4([node]):
+            return _q4_weight(g, [node], device, interleave=interleave)
+        return _fp4_weight(g, [node], device, interleave=interleave) if keep_fp4 and _is_fp4([node]) else None
 
     def linear_node(prefix: str, *names):
         for nm in names:
@@ -434,9 +463,8 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
             # attention projections: packed or separate
             qkv = linear_node(f"{n}/attn/", "qkv_proj")
             if qkv is not None:
-                if keep_q4 and _is_q4([qkv]):
-                    lw.qkv_w = _q4_weight(g, [qkv], device)
-                else:
+                lw.qkv_w = packed_weight(qkv)
+                if lw.qkv_w is None:
                     w = _linear_weight(g, qkv, dtype, device)
                     lw.qkv_w = shard_rows(w, [q_rows, k_rows, v_rows])
                 badd = g.by_name.get(f"{n}/attn/qkv_proj/Add")
@@ -444,22 +472,22 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
                     b = g.tensor(badd.inputs[1])
                     lw.qkv_b = shard_rows(b, [q_rows, k_rows, v_rows]).to(device=device, dtype=dtype)
             else:
-                ws, bs = [], []
+                ws, bs, nodes = [], [], [linear_node(f"{n}/attn/", nm) for nm in ("q_proj", "k_proj", "v_proj")]
+                stacked = keep_fp4 and _is_fp4(nodes)
                 for nm, rows in (("q_proj", slice(tpr * hq_l * D, (tpr + 1) * hq_l * D)),
                                  ("k_proj", slice(tpr * hkv_l * D, (tpr + 1) * hkv_l * D)),
                                  ("v_proj", slice(tpr * hkv_l * D, (tpr + 1) * hkv_l * D))):
-                    node = linear_node(f"{n}/attn/", nm)
-                    ws.append(_linear_weight(g, node, dtype, device, rows=rows if tpn > 1 else None))
+                    if not stacked:
+                        ws.append(_linear_weight(g, linear_node(f"{n}/attn/", nm), dtype, device, rows=rows if tpn > 1 else None))
                     badd = g.by_name.get(f"{n}/attn/{nm}/Add")
                     if badd is not None:
                         b = g.tensor(badd.inputs[1])
                         bs.append((b[rows] if tpn > 1 else b).to(device=device, dtype=dtype))
-                lw.qkv_w = torch.cat(ws, 0).contiguous()
+                lw.qkv_w = _fp4_weight(g, nodes, device) if stacked else torch.cat(ws, 0).contiguous()
                 lw.qkv_b = torch.cat(bs, 0).contiguous() if bs else None
             o = linear_node(f"{n}/attn/", "o_proj")
-            if keep_q4 and _is_q4([o]):
-                lw.o_w = _q4_weight(g, [o], device)
-            else:
+            lw.o_w = packed_weight(o)
+            if lw.o_w is None:
                 lw.o_w = _linear_weight(g, o, dtype, device, cols=slice(tpr * hq_l * D, (tpr + 1) * hq_l * D) if tpn > 1 else None)
             gate = g.find(f"{n}/attn/gate_proj/", ops=LINEAR_OPS)
             if gate is not None:
@@ -610,8 +638,12 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
                 lw.exp_blocked = True
         elif not arch.mlp_gated:
             i_rows = slice(tpr * i_l, (tpr + 1) * i_l)
-            lw.fc1_w = _linear_weight(g, linear_node(f"{n}/mlp/", "fc1"), dtype, device, rows=i_rows if tpn > 1 else None)
-            lw.fc2_w = _linear_weight(g, linear_node(f"{n}/mlp/", "fc2"), dtype, device, cols=i_rows if tpn > 1 else None)
+            fc1, fc2 = linear_node(f"{n}/mlp/", "fc1"), linear_node(f"{n}/mlp/", "fc2")
+            if keep_fp4 and _is_fp4([fc1, fc2]):
+                lw.fc1_w, lw.fc2_w = _fp4_weight(g, [fc1], device), _fp4_weight(g, [fc2], device)
+            else:
+                lw.fc1_w = _linear_weight(g, fc1, dtype, device, rows=i_rows if tpn > 1 else None)
+                lw.fc2_w = _linear_weight(g, fc2, dtype, device, cols=i_rows if tpn > 1 else None)
             b1, b2 = g.by_name.get(f"{n}/mlp/fc1/Add"), g.by_name.get(f"{n}/mlp/fc2/Add")
             if b1 is not None:
                 lw.fc1_b = _vec(g, b1.inputs[1], dtype, device, i_rows if tpn > 1 else None)
@@ -620,9 +652,13 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
         else:
             gu = linear_node(f"{n}/mlp/", "gate_up_proj")
             g_rows, u_rows = slice(tpr * i_l, (tpr + 1) * i_l), slice(I + tpr * i_l, I + (tpr + 1) * i_l)
-            if gu is not None and keep_q4 and _is_q4([gu]):
-                il = arch.activation == "silu" and I % 64 == 0
-                lw.gate_up_w = _q4_weight(g, [gu], device, interleave=il)
+            il = arch.activation == "silu" and I % 64 == 0
+            gates = [linear_node(f"{n}/mlp/", nm) for nm in ("gate_proj", "up_proj")] if gu is None else [gu]
+            if gu is not None:
+                lw.gate_up_w = packed_weight(gu, il)
+            elif keep_fp4 and _is_fp4(gates):
+                lw.gate_up_w = _fp4_weight(g, gates, device, interleave=il)
+            if lw.gate_up_w is not None:
                 lw.gate_up_interleaved = il
                 badd = g.by_name.get(f"{n}/mlp/gate_up_proj/Add")
                 if badd is not None:
@@ -647,9 +683,8 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
                     lw.gate_up_b = interleave_gate_up(lw.gate_up_b)
                 lw.gate_up_interleaved = True
             dn = linear_node(f"{n}/mlp/", "down_proj")
-            if keep_q4 and _is_q4([dn]):
-                lw.down_w = _q4_weight(g, [dn], device)
-            else:
+            lw.down_w = packed_weight(dn)
+            if lw.down_w is None:
                 lw.down_w = _linear_weight(g, dn, dtype, device, cols=g_rows if tpn > 1 else None)
             dadd = g.by_name.get(f"{n}/mlp/down_proj/Add")
             if dadd is not None:
@@ -668,9 +703,8 @@ def load_decoder(model_dir: str, cfg, device, dtype, tp=None, decoder: Optional[
         model.vocab_shard = (rows.start, rows.stop, per)
     else:
         rows = None
-    if keep_q4 and _is_q4([head]):
-        model.lm_head_w = _q4_weight(g, [head], device)
-    else:
+    model.lm_head_w = packed_weight(head)
+    if model.lm_head_w is None:
         model.lm_head_w = _linear_weight(g, head, dtype, device, rows=rows)
     hadd = g.by_name.get("/lm_head/Add")
     if hadd is not None:

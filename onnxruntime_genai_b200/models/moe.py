@@ -32,6 +32,8 @@ from .arch import MoeSpec
 
 # OGB_MOE_ROW_MAP=0: the token rows of packed experts are gathered into a copy instead of being read through the row map
 _ROW_MAP = os.environ.get("OGB_MOE_ROW_MAP", "1") != "0"
+# OGB_MOE_FEW=1: steps of a few tokens run a whole layer of routed experts in two kernels (ops.moe_few_tokens)
+_FEW = os.environ.get("OGB_MOE_FEW", "0") == "1"
 
 
 def swiglu_interleaved(gu: torch.Tensor, alpha: float, limit: float) -> torch.Tensor:
@@ -210,6 +212,15 @@ def _forward_simt(model, lw, x):
     return ops.PendingCombine(ops.moe_gemm_simt(h, lw.exp_down_w, plan), plan, shared_expert(lw, x, sp) if lw.shared_gate_up_w is not None else None)
 
 
+def _few_ok(lw, sp: MoeSpec, x: torch.Tensor) -> bool:
+    """The layer and its rows are among those that ops.moe_few_tokens takes: routing by a softmax, gated experts, none of them shared."""
+    if not _FEW or x.shape[0] > ops.MOE_FEW_TOKENS or x.shape[0] == 0 or sp.weights not in _TOPK_MODES or not sp.gated or lw.exp_shared:
+        return False
+    packed = isinstance(lw.exp_gate_up_w, ops.Fp4Experts)
+    return (lw.shared_gate_up_w is None and x.dtype == lw.router_w.dtype == torch.bfloat16 and (packed or lw.exp_gate_up_w.dtype == torch.bfloat16) and
+            (not packed or lw.exp_gate_up_w.half == lw.exp_down_w.half))
+
+
 def moe_forward(model, lw, x: torch.Tensor, defer: bool = False):
     """defer: the caller folds the combine step into the residual add + norm that follows (`ops.norm_moe_combine`); the
     result is then an `ops.PendingCombine` when the layer ran on the device path of a single rank."""
@@ -219,6 +230,9 @@ def moe_forward(model, lw, x: torch.Tensor, defer: bool = False):
         # token-sharded expert parallelism: dispatch / combine all-to-all, the output is complete on every rank
         from ..parallel.ep import moe_all_to_all
         return moe_all_to_all(model, lw, x)
+    if fast and model.tp.size == 1 and _few_ok(lw, sp, x):
+        return ops.moe_few_tokens(x, lw.router_w, lw.router_b, lw.exp_gate_up_w, lw.exp_gate_up_b, lw.exp_down_w, lw.exp_down_b, sp.top, sp.weights, sp.act,
+                                  sp.alpha, sp.limit)
     if fast:
         return _forward_device(model, lw, x, defer and model.tp.size == 1) if model.tp.size == 1 else model.tp.reduce(_forward_device(model, lw, x))
     if x.is_cuda and lw.moe is not None and defer and model.tp.size == 1:
