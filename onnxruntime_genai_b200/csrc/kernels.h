@@ -352,6 +352,7 @@ int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T
 // ---- moe_few.cu (a whole expert layer for up to eight tokens; rule: mode of ogb_moe_topk; weights 0: bf16, 1 / 2: packed MXFP4 in its fp16 / bf16 form;
 // act 1: silu(gate) * up, 2: clamped SwiGLU; gate_up in blocks of 64 gate + 64 up rows)
 long long ogb_moe_few_scratch_bytes(int T, int top, int I);     // -1: refused
+int ogb_moe_few_takes(int T, int H, int I, int E, int top);     // whether ogb_moe_few_tokens has a layer of these sizes
 int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b, const void* down,
                        const void* down_b, void* out, int T, int H, int I, int E, int top, int rule, int weights, int act, float alpha, float limit,
                        void* scratch, int* status, int sm_count, void* stream);

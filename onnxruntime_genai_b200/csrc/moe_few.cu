@@ -20,6 +20,7 @@
 
 #include "kernels.h"
 #include "packed_weights.cuh"
+#include "tensor_map.cuh"
 
 namespace ogb {
 
@@ -741,21 +742,30 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
 }
 
 // --------------------------------------------------------------------------------- host side
-bool MakeMapBf16(CUtensorMap* out, const void* ptr, int rows, int cols, int ld, int box_rows);  // gemm_tcgen05.cu
+// Shared memory of the first kernel besides its ring: rows and logits of all tokens
+static size_t few_fixed(int T, int H, int E) {
+  return 1024 + sizeof(FewShared) + (size_t(T) * E * 4 + 15) / 16 * 16 + size_t(T) * ((H + 63) / 64 * 64 + 32) * 2;
+}
+// A place in the ring for each team (of the largest stage) has to be left.
+static bool few_fits(int T, int H, int E) {
+  using Tile = FewTile<FEW_BF16, 128>;
+  static_assert(Tile::CHUNKS * Tile::BYTES >= FewTile<FEW_FP4_F16, 128>::CHUNKS * FewTile<FEW_FP4_F16, 128>::BYTES, "the largest stage");
+  return H <= 65536 && few_fixed(T, H, E) + Tile::TEAMS * Tile::CHUNKS * Tile::BYTES <= FEW_SMEM_ONE;
+}
 
 template <int W>
 static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
   using Tile = FewTile<W, 128>;
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
-  const int Hp = (p.H + 63) / 64 * 64;
-  const size_t fixed = 1024 + sizeof(FewShared) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16 + size_t(p.T) * (Hp + 32) * 2;
+  const size_t fixed = few_fixed(p.T, p.H, p.E);
   // Two CTAs an SM where that leaves each a ring of 32 KiB: more warps to expand and multiply; else one with what there is.
   const int two = fixed + 32 * 1024 <= FEW_SMEM_TWO;
   const size_t room = two ? FEW_SMEM_TWO : FEW_SMEM_ONE;
-  if (fixed + Tile::TEAMS * STAGE > room) return -5;
   p.stages = Tile::ring(int(room - fixed), STAGE);
   CUtensorMap gate_up = {}, down = {};
-  if (W == FEW_BF16 && (!MakeMapBf16(&gate_up, p.gate_up, p.E * 2 * p.I, p.H, p.H, 128) || !MakeMapBf16(&down, p.down, p.E * p.H, p.I, p.I, FEW_DOWN_ROWS))) return -2;
+  if (W == FEW_BF16 && (!encode_map_2d(&gate_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.gate_up, uint64_t(p.E) * 2 * p.I, p.H, uint64_t(p.H) * 2, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
+                        !encode_map_2d(&down, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.down, uint64_t(p.E) * p.H, p.I, uint64_t(p.I) * 2, FEW_DOWN_ROWS, 64, CU_TENSOR_MAP_SWIZZLE_128B)))
+    return -2;
   static bool configured[OGB_MAX_DEVICES] = {}, configured_down[OGB_MAX_DEVICES] = {};
   if (!set_max_dyn_smem(few_gate_up_kernel<W>, int(FEW_SMEM_ONE), configured) || !set_max_dyn_smem(few_down_kernel<W>, FEW_DOWN_RING + 1024, configured_down)) return -3;
   // Both kernels are launched behind the complete kernels in front of them: CTAs that come in as others leave are placed so that some clusters find no room until the
@@ -800,11 +810,15 @@ OGB_API long long ogb_moe_few_scratch_bytes(int T, int top, int I) {
   return T < 1 || T > FEW_TOKENS || top < 1 || top > FEW_TOP || I < 1 ? -1 : (long long)sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL + (long long)T * top * I * 2;
 }
 
+OGB_API int ogb_moe_few_takes(int T, int H, int I, int E, int top) {
+  return ogb_moe_few_scratch_bytes(T, top, I) >= 0 && H >= 1 && H % 8 == 0 && I % 64 == 0 && E >= top && E <= FEW_EXPERTS && few_fits(T, H, E);
+}
+
 OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router, const void* router_b, const void* gate_up, const void* gate_up_b,
                                const void* down, const void* down_b, void* out, int T, int H, int I, int E, int top, int rule, int weights, int act,
                                float alpha, float limit, void* scratch, int* status, int sm_count, void* stream) {
-  if (ogb_moe_few_scratch_bytes(T, top, I) < 0 || !x || !router || !gate_up || !down || !out || !scratch || H < 1 || H % 8 || E < top || E > FEW_EXPERTS ||
-      I % 64 || (weights != FEW_BF16 && H % 64) || rule < 0 || rule > 2 || weights < 0 || weights > 2 || (act != 1 && act != 2)) return -1;
+  if (!ogb_moe_few_takes(T, H, I, E, top) || !x || !router || !gate_up || !down || !out || !scratch || (weights != FEW_BF16 && H % 64) || rule < 0 || rule > 2 ||
+      weights < 0 || weights > 2 || (act != 1 && act != 2)) return -1;
   if ((reinterpret_cast<uintptr_t>(x) | uintptr_t(ldx * 2) | reinterpret_cast<uintptr_t>(router) | reinterpret_cast<uintptr_t>(gate_up) | reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(scratch)) & 15)
     return -1;
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,

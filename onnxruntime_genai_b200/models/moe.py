@@ -218,7 +218,8 @@ def _few_ok(lw, sp: MoeSpec, x: torch.Tensor) -> bool:
         return False
     packed = isinstance(lw.exp_gate_up_w, ops.Fp4Experts)
     return (lw.shared_gate_up_w is None and x.dtype == lw.router_w.dtype == torch.bfloat16 and (packed or lw.exp_gate_up_w.dtype == torch.bfloat16) and
-            (not packed or lw.exp_gate_up_w.half == lw.exp_down_w.half))
+            (not packed or lw.exp_gate_up_w.half == lw.exp_down_w.half) and
+            ops.moe_few_takes(x.shape[0], x.shape[1], lw.exp_gate_up_w.shape[1] // 2, sp.experts, sp.top))
 
 
 def moe_forward(model, lw, x: torch.Tensor, defer: bool = False):

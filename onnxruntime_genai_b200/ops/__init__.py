@@ -973,6 +973,11 @@ _FEW_RULES = {"selected": 0, "all": 1, "renormed": 2}
 _FEW_ACTS = {"silu": 1, "clamped": 2}
 
 
+def moe_few_takes(T: int, H: int, I: int, E: int, top: int) -> bool:
+    """Whether moe_few_tokens has a layer of these sizes (rows and logits of all tokens stand in shared memory: 8 tokens of up to 10000 columns or so)."""
+    return bool(_lib.lib().ogb_moe_few_takes(T, H, I, E, top))
+
+
 def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, top: int, weights: str = "selected", act: str = "silu", alpha: float = 1.0,
                    limit: float = 0.0):
     """A whole mixture-of-experts layer for up to eight tokens: router product, choice of `top` experts per token (the largest logits, the lowest index among
@@ -1008,6 +1013,8 @@ def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, 
     if x.stride(1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     out = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    if T * H > 32768 and not moe_few_takes(T, H, I, E, top):
+        raise ValueError(f"moe_few_tokens: {T} rows of {H} columns and the logits of {E} experts do not fit shared memory")
     scratch = torch.empty(_lib.lib().ogb_moe_few_scratch_bytes(T, top, I), dtype=torch.uint8, device=x.device)
     ws = workspace(x.device)
     _call_on(ws.index, "ogb_moe_few_tokens", x.data_ptr(), x.stride(0), router_w.data_ptr(), _ptr(router_b), (gate_up_w.packed if packed else gate_up_w).data_ptr(),

@@ -185,6 +185,7 @@ _SIGS = {
     "ogb_linear_fp4": (c_int, [_P, c_longlong, c_int, _P, c_int, _P, c_int, c_int, c_int, _P, c_longlong, c_int, c_int, _P, _P, c_longlong, c_int, _P, c_int,
                                _P]),
     "ogb_moe_few_scratch_bytes": (c_longlong, [c_int, c_int, c_int]),
+    "ogb_moe_few_takes": (c_int, [c_int, c_int, c_int, c_int, c_int]),
     "ogb_moe_few_tokens": (c_int, [_P, c_longlong, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, _P, _P,
                                    c_int, _P]),
     "ogb_verify_greedy": (c_int, [_P, _P, c_int, _P, _P, _P]),

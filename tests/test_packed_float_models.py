@@ -80,6 +80,10 @@ def test_layers_the_few_token_form_takes(monkeypatch):
     assert not moe._few_ok(lw, spec, x[:0]) and not moe._few_ok(lw, spec, torch.zeros(9, 64, dtype=torch.bfloat16)) and not moe._few_ok(lw, spec, x.float())
     for other in (dict(weights="sigmoid"), dict(weights="sparse_mixer"), dict(act="relu2")):
         assert not moe._few_ok(lw, moe.MoeSpec(8, 2, **other), x)
+    wide = torch.zeros(8, 1 << 14, dtype=torch.bfloat16)
+    lw.exp_gate_up_w = torch.zeros(1, 256, 1, dtype=torch.bfloat16).expand(8, 256, 1 << 14)
+    assert moe._few_ok(lw, spec, wide[:1]) and not moe._few_ok(lw, spec, wide)           # eight rows of it do not fit shared memory
+    lw.exp_gate_up_w = torch.zeros(8, 256, 64, dtype=torch.bfloat16)
     lw.exp_shared = True
     assert not moe._few_ok(lw, spec, x)
     lw.exp_shared, lw.shared_gate_up_w = False, torch.zeros(2, 2)
