@@ -65,15 +65,11 @@ template <> struct Raw8<__nv_bfloat16> {
     }
   }
   __device__ __forceinline__ void zero() { q = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ uint32_t largest() const {        // bits of the largest magnitude, as fp32
-    const uint32_t m = 0x7fff7fffu, a = max2(max2(q.x & m, q.y & m), max2(q.z & m, q.w & m));
-    return max(a & 0xffff0000u, a << 16);
+  __device__ __forceinline__ uint32_t largest() const {        // bits of the largest magnitude, as fp32 (a NaN: of a NaN)
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(part(q.x), part(q.y)), __hmax2_nan(part(q.z), part(q.w)));
+    return uint32_t(__bfloat16_as_ushort(__hmax_nan(m.x, m.y))) << 16;
   }
-  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-  }
+  static __device__ __forceinline__ __nv_bfloat162 part(uint32_t w) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)); }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -115,7 +111,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
   pdl_wait();
   pdl_launch_dependents();     // after the wait: whoever starts now may read what the kernels before this one wrote (linear_fp4.cu does)
   Raw8<T> held[HELD];
-  uint32_t top = 0;
+  uint32_t top = 0, most[HELD];
   auto fetch = [&](int kb) {
     Raw8<T> r;
     const int k = kb * FP4_KB + lane * 8;
@@ -125,7 +121,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
 #pragma unroll
   for (int i = 0; i < HELD; ++i) held[i] = fetch(first + i * wpr);
 #pragma unroll
-  for (int i = 0; i < HELD; ++i) top = max(top, held[i].largest());
+  for (int i = 0; i < HELD; ++i) {
+    most[i] = held[i].largest();
+    top = max(top, most[i]);
+  }
   for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) top = max(top, fetch(kb).largest());
   top = __reduce_max_sync(0xffffffffu, top);
   if (wpr > 1) {
@@ -139,28 +138,38 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
   const float s = pow2(re), over = pow2(-re);
   if (first == 0 && lane == 0) out.row_scale[row] = bad ? __uint_as_float(0x7fc00000u) : s;
 
-  constexpr int PER = FORM == FP4_NV ? 2 : 4;                              // lanes of a block; four blocks' scales are one word
+  constexpr int PER = FORM == FP4_NV ? 2 : 4;                              // lanes of a block
   uint8_t* codes_to = out.codes + fp4_code_at(out, first, row, lane >> 2) + (lane & 3) * 4;
-  uint8_t* scales_to = out.scales + fp4_scale_at(out, FORM, first, row, lane / (4 * PER), 0);
+  uint8_t* scales_to = out.scales + fp4_scale_at(out, FORM, first, row, lane / (4 * PER), lane / PER & 3);
   const long long codes_step = (long long)wpr * out.padded * 128, scales_step = (long long)wpr * (out.padded >> 7) * (fp4_steps(FORM) * FP4_SCALE_STEP);
-  auto emit = [&](const Raw8<T>& r) {
+  auto emit = [&](const Raw8<T>& r, uint32_t m) {
     float v[8];
-    uint32_t m = r.largest();
     r.get(v);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     uint32_t code;
     if (FORM == FP4_NV) {
-      // Quotients are products with the rounded reciprocal and one correction by the exact remainder, so that one that is a tie comes out as that tie.  The powers
-      // of two of the row's scale change no rounding.
+      // Quotients are products with a reciprocal.  One that is a tie has to come out as that tie, and one that is not on its side of it; the powers of two of
+      // the row's scale change no rounding.
       constexpr float sixth = 1.f / 6.f;
       const float t = __uint_as_float(m) * over, h = t * sixth;
-      code = bad ? 0u : e4m3_of(fmaf(fmaf(-h, 6.f, t), sixth, h));
-      const float sc = fp4_scale_nv(code), by = sc * s, near = __fdividef(1.f, sc);
-      const float inv = code ? fmaf(fmaf(-sc, near, 1.f), near, near) * over : 0.f;      // (a Newton step makes the approximate reciprocal the nearest one)
+      if constexpr (sizeof(T) == 2) {
+        // Of numbers of eight bits: a sixth of such a number is a tie of e4m3 only where the product with the rounded 1/6 comes out exact (tested for all of
+        // them), and a quotient by a scale of four bits is a tie or at least 2^-10 away from it, so that rounding it to whole 2^-14, by an addition, puts it right.
+        constexpr float grid = 768.f;                                       // 1.5 * 2^9; quotients are at most 9
+        code = bad ? 0u : e4m3_of(h);
+        const float inv = code ? __fdividef(1.f, fp4_scale_nv(code)) * over : 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float q = v[i] * inv;
-        v[i] = fmaf(fmaf(-q, by, v[i]), inv, q);
+        for (int i = 0; i < 8; ++i) v[i] = __fsub_rn(fmaf(v[i], inv, grid), grid);
+      } else {
+        // Else: one correction by the exact remainder, with reciprocals that a Newton step makes the nearest ones.
+        code = bad ? 0u : e4m3_of(fmaf(fmaf(-h, 6.f, t), sixth, h));
+        const float sc = fp4_scale_nv(code), by = sc * s, near = __fdividef(1.f, sc);
+        const float inv = code ? fmaf(fmaf(-sc, near, 1.f), near, near) * over : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float q = v[i] * inv;
+          v[i] = fmaf(fmaf(-q, by, v[i]), inv, q);
+        }
       }
     } else {
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -173,15 +182,17 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 2) quantize_fp4_
       for (int i = 0; i < 8; ++i) v[i] *= inv;
     }
     *reinterpret_cast<uint32_t*>(codes_to) = bad ? 0u : e2m1x8(v);
-    const uint32_t c1 = __shfl_down_sync(0xffffffffu, code, PER), c2 = __shfl_down_sync(0xffffffffu, code, 2 * PER), c3 = __shfl_down_sync(0xffffffffu, code, 3 * PER);
-    if (lane % (4 * PER) == 0) *reinterpret_cast<uint32_t*>(scales_to) = code | c1 << 8 | c2 << 16 | c3 << 24;
+    if (lane % PER == 0) *scales_to = uint8_t(code);
     codes_to += codes_step;
     scales_to += scales_step;
   };
 #pragma unroll
   for (int i = 0; i < HELD; ++i)
-    if (first + i * wpr < out.num_kb) emit(held[i]);
-  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) emit(fetch(kb));
+    if (first + i * wpr < out.num_kb) emit(held[i], most[i]);
+  for (int kb = first + HELD * wpr; kb < out.num_kb; kb += wpr) {
+    const Raw8<T> r = fetch(kb);
+    emit(r, r.largest());
+  }
 }
 
 // A warp reads four rows of a k-block (512 bytes of codes), eight elements a lane and row.

@@ -178,3 +178,22 @@ def test_refusals_of_device_tensors():
         ops.linear(x, w, out=torch.zeros(2, 64, device=DEV))
     with pytest.raises(ValueError, match="residual"):
         ops.linear(x, w, residual=torch.zeros(2, 64, dtype=torch.float16, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_of_every_significand(dtype):
+    """Blocks whose largest magnitude takes every significand of bf16 at many sizes under the row's largest, and whose other numbers are whole eighths of an
+    e4m3 scale's significand times ties of e2m1, or next to those."""
+    g = torch.Generator().manual_seed(12)
+    rows, blocks = 128, 48
+    x = torch.zeros(rows, blocks, 16)
+    top = torch.arange(128, 256)[:, None] * 2.0 ** -torch.arange(blocks)[None, :].div(2, rounding_mode="floor").float()
+    x[..., 0] = top * torch.where(torch.rand(rows, blocks, generator=g) < 0.5, -1.0, 1.0)
+    tie = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])[torch.randint(0, 7, (rows, blocks, 15), generator=g)]
+    scale = (top / 6).to(torch.float8_e4m3fn).float()[..., None]                       # (of a row scale of one; others move it by a power of two)
+    near = (tie * scale).to(torch.bfloat16)
+    bits = (near.view(torch.int16) + torch.randint(-1, 2, near.shape, generator=g).to(torch.int16)).clamp(min=0)
+    x[..., 1:] = torch.minimum(bits.view(torch.bfloat16).float(), top[..., None]) * torch.where(torch.rand(rows, blocks, 15, generator=g) < 0.5, -1.0, 1.0)
+    x = x.view(rows, -1).to(dtype)
+    for row in (x, x * 2.0 ** 7, x * 2.0 ** -9):
+        assert torch.equal(ops.quantize_fp4(row.to(DEV)).dequantize().cpu(), fp4_matrix.quantize(row, "nvfp4").dequantize())
