@@ -437,7 +437,7 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
 
 def _call_on(index: int, entry: str, *args):
     """Runs an entry point of the kernel library on device `index`, on that device's current stream (the last argument)."""
-    if index != torch.cuda.current_device():
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
             return _call_on(index, entry, *args)
     _lib.check(getattr(_lib.lib(), entry)(*args, torch._C._cuda_getCurrentRawStream(index)), entry)
