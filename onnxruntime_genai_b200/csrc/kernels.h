@@ -344,7 +344,9 @@ int ogb_paged_attention_kv8(const void* q, int q_stride, const void* k_cache, co
 long long ogb_fp4_matrix_bytes(int rows, int K, int form);      // of one buffer of codes, block scales and row scales; -1: refused
 int ogb_quantize_fp4(const void* x, long long ldx, int x_fp32, int rows, int K, int form, void* data, void* stream);
 int ogb_dequantize_fp4(const void* data, int rows, int K, int form, void* out, long long ldo, int out_fp32, void* stream);
-// x != null: these rows are quantised into a_data first; null: a_data holds quantised rows.  pair: silu(gate) * up of blocks of 64 + 64 weight rows
+// Whether ogb_linear_fp4 has a form for T rows that quantises them by itself
+int ogb_linear_fp4_own_rows(int T, int N, int K, int sm_count);
+// x != null: these rows are quantised, into a_data or (null, where there is a form for it) by the product itself; null: a_data holds quantised rows.  pair: silu(gate) * up of blocks of 64 + 64 weight rows
 int ogb_linear_fp4(const void* x, long long ldx, int x_fp32, void* a_data, int T, const void* w_data, int N, int K, int form, void* out, long long ldc,
                    int out_fp32, int pair, const void* bias, const void* residual, long long ldr, int res_fp32, int* status, int sm_count,
                    void* stream);

@@ -18,6 +18,9 @@ struct Fp4LinearArgs {
   int whole;                    // every eight columns of an output and residual row are aligned for 16-byte accesses
   int splits, kb_per_split;     // parts of the k-blocks, none of them empty
   int stages;
+  const void* x;                // rows that the kernel quantises itself (else they are in `a`), K of them and ldx apart; x_vec: every eight aligned for 16-byte loads
+  long long ldx;
+  int K, x_fp32, x_vec;
   int early;                    // weights may be fetched before the kernel in front has finished (it does not write them, nor do those before it)
   int* status;
   int pdl;

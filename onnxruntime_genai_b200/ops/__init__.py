@@ -501,15 +501,16 @@ def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=N
         return y if out is None else out.copy_(y)
     if out is None:
         out = torch.empty(T, n_out, dtype=torch.float32 if out_fp32 else torch.bfloat16, device=dev)
+    ws = workspace(dev)
     if given:
         rows, ldx, x32, a = None, 0, False, x.data
     else:
         if x.stride(1) != 1:
             x = x.contiguous()
-        rows, ldx, x32 = x.data_ptr(), x.stride(0), x.dtype == torch.float32
-        a = torch.empty(fp4_matrix.matrix_bytes(T, K, w.form), dtype=torch.uint8, device=dev)
-    ws = workspace(dev)
-    _call_on(ws.index, "ogb_linear_fp4", rows, ldx, x32, a.data_ptr(), T, data.data_ptr(), N, K, fp4_matrix.FORMS[w.form], out.data_ptr(), out.stride(0), out_fp32, pair,
+        rows, ldx, x32, a = x.data_ptr(), x.stride(0), x.dtype == torch.float32, None
+        if T > 2 or not _lib.lib().ogb_linear_fp4_own_rows(T, N, K, ws.sm_count):
+            a = torch.empty(fp4_matrix.matrix_bytes(T, K, w.form), dtype=torch.uint8, device=dev)
+    _call_on(ws.index, "ogb_linear_fp4", rows, ldx, x32, _ptr(a), T, data.data_ptr(), N, K, fp4_matrix.FORMS[w.form], out.data_ptr(), out.stride(0), out_fp32, pair,
              _ptr(bias), _ptr(residual), 0 if residual is None else residual.stride(0), residual is not None and residual.dtype == torch.float32, ws.status, ws.sm_count)
     return out
 

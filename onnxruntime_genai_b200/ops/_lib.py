@@ -182,6 +182,7 @@ _SIGS = {
     "ogb_fp4_matrix_bytes": (c_longlong, [c_int, c_int, c_int]),
     "ogb_quantize_fp4": (c_int, [_P, c_longlong, c_int, c_int, c_int, c_int, _P, _P]),
     "ogb_dequantize_fp4": (c_int, [_P, c_int, c_int, c_int, _P, c_longlong, c_int, _P]),
+    "ogb_linear_fp4_own_rows": (c_int, [c_int, c_int, c_int, c_int]),
     "ogb_linear_fp4": (c_int, [_P, c_longlong, c_int, _P, c_int, _P, c_int, c_int, c_int, _P, c_longlong, c_int, c_int, _P, _P, c_longlong, c_int, _P, c_int,
                                _P]),
     "ogb_moe_few_scratch_bytes": (c_longlong, [c_int, c_int, c_int]),

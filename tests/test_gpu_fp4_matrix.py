@@ -197,3 +197,37 @@ def test_rows_of_every_significand(dtype):
     x = x.view(rows, -1).to(dtype)
     for row in (x, x * 2.0 ** 7, x * 2.0 ** -9):
         assert torch.equal(ops.quantize_fp4(row.to(DEV)).dequantize().cpu(), fp4_matrix.quantize(row, "nvfp4").dequantize())
+
+
+@pytest.mark.parametrize("form", ["nvfp4", "mxfp4"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,N,K", [(1, 128, 32), (1, 6144, 4096), (1, 28672, 4096), (1, 300, 8192), (1, 300, 16384), (1, 18944, 512), (2, 1000, 2880), (2, 6144, 4096),
+                                   (2, 200, 8192), (3, 130, 288), (1, 14208, 6656)])
+def test_rows_quantised_by_the_product(T, N, K, dtype, form):
+    """Few rows that are not quantised yet: the same numbers as through the rows' own kernel, whichever of the two takes them."""
+    wide = torch.full((T, K + 5), 9.0)
+    wide[:, 1:K + 1] = rows_of("wide", T, K, torch.bfloat16).float()
+    if T > 1:
+        wide[1, 1 + K // 2] = math.nan
+    x = wide.to(dtype).to(DEV)[:, 1:K + 1]
+    w = weight(N, K, form)
+    want = ops.linear(ops.quantize_fp4(x, form), w, out_fp32=True)
+    for rows in (x, x.contiguous()):
+        got = ops.linear(rows, w, out_fp32=True)
+        assert torch.equal(got.nan_to_num(5.0), want.nan_to_num(5.0)) and torch.equal(torch.isnan(got), torch.isnan(want))
+    gated = weight(128 * (N // 128), K, form, interleaved=True) if N >= 128 else None
+    if gated is not None:
+        assert torch.equal(ops.gate_up_act(x, gated).nan_to_num(5.0), ops.gate_up_act(ops.quantize_fp4(x, form), gated).nan_to_num(5.0))
+    ops.check_kernel_status()
+
+
+def test_rows_that_are_not_numbers_or_zero_and_the_product_that_quantises():
+    w = weight(384, 512, "nvfp4")
+    for fill in (0.0, math.inf, -math.inf, math.nan):
+        x = rows_of("normal", 2, 512, torch.bfloat16).to(DEV)
+        other = ops.linear(x, w)[0]
+        x[1, 300:] = fill
+        if fill == 0.0:
+            x[1] = 0.0
+        got = ops.linear(x, w)
+        assert torch.equal(got[0], other) and bool((got[1] == 0).all() if fill == 0.0 else torch.isnan(got[1]).all())
