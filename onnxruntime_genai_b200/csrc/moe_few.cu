@@ -245,32 +245,29 @@ static __device__ __noinline__ bool few_wait_slow(FewBars* b, uint32_t full, uin
   *reinterpret_cast<volatile int*>(&b->abort) = 1;
   return false;
 }
-template <int STAGE>
-struct FewReader {                     // the multiplying side
+template <int STAGE, int TEAMS>
+struct FewReader {                     // the multiplying side: every TEAMS-th stage
   FewBars* b;
-  uint32_t base, data, full, last = 0, ph = 0, end;      // addresses: first stage, this stage, its barrier, the barrier of the stage read before; end of the ring
-  __device__ __forceinline__ FewReader(FewBars* bars, const void* ring, int stages)
-      : b(bars), base(smem_u32(ring)), data(base), full(smem_u32(bars->full)), end(base + stages * STAGE) {}
+  uint32_t data, full, ph = 0, end, ring;                // addresses: this stage, its barrier; end of the ring, its bytes
+  __device__ __forceinline__ FewReader(FewBars* bars, const void* first, int stages, int team)
+      : b(bars), data(smem_u32(first) + team * STAGE), full(smem_u32(bars->full) + team * 8), end(smem_u32(first) + stages * STAGE), ring(stages * STAGE) {}
   __device__ __forceinline__ void next() {
-    data += STAGE;
-    full += 8;
-    if (data == end) { data = base; full = smem_u32(b->full); ph ^= 1; }
+    data += TEAMS * STAGE;
+    full += TEAMS * 8;
+    if (data >= end) { data -= ring; full -= ring / STAGE * 8; ph ^= 1; }
   }
   // false: the wait ran out; the warp goes through its loop without reading, so that it meets the barriers that the others wait at
   __device__ __forceinline__ bool wait(int* status) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(full), "r"(ph) : "memory");
-    if (!__all_sync(0xffffffffu, ok) && !few_wait_slow(b, full, ph, status)) return false;
-    last = full + sizeof(uint64_t) * FEW_STAGES;         // (the stage's `empty`)
-    return true;
+    return __all_sync(0xffffffffu, ok) || few_wait_slow(b, full, ph, status);
   }
-  // Hands back the stage that this warp has read; called in the next turn of the loop.  Directly behind its products the arrival could overtake reads of shared memory
-  // that are still on their way (seen as single wrong rows: nothing makes the arrival wait for loads whose values are used later); a turn later the products have
-  // been issued, for which all their operands had to be there.
-  __device__ __forceinline__ void release(int lane) {
+  // Hands back the stage.  An arrival does not wait for reads of shared memory that are still on their way (seen as single wrong rows), so it stands behind the sums:
+  // they have been issued then, for which all that was read had to be there.
+  __device__ __forceinline__ void release(int lane, float (&acc)[2][4]) {
+    asm volatile("" : "+f"(acc[0][0]), "+f"(acc[0][1]), "+f"(acc[0][2]), "+f"(acc[0][3]), "+f"(acc[1][0]), "+f"(acc[1][1]), "+f"(acc[1][2]), "+f"(acc[1][3]));
     __syncwarp();
-    if (last && lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(last) : "memory");
-    last = 0;
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + uint32_t(sizeof(uint64_t)) * FEW_STAGES) : "memory");       // (the stage's `empty`)
   }
 };
 
@@ -553,24 +550,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     const int team = warp >> 2;
     const uint32_t place = Tile::place((warp & 3) * 16 + g, g, q), scales = Tile::scales((warp & 3) * 16 + g);
     float acc[2][4] = {};
-    FewReader<STAGE> r(&sh.bars, ring, p.stages);
-    int item = lo / steps, c = (lo - item * steps) * Tile::CHUNKS, parity = 0;
-    bool whole = c == 0, ok = true;
-    for (int i = lo; i < hi; ++i, parity ^= 1) {
-      r.release(lane);
-      if (parity == team && ok && (ok = r.wait(p.status))) {
-        const uint32_t x = xt + c * 128;
-        uint4 b[2] = {lds128<0>(x), lds128<64>(x)};
-        Tile::mma(acc, r.data + place, r.data + scales, b);
-        if (Tile::CHUNKS == 2 && c + 1 < chunks) {
-          b[0] = lds128<128>(x);
-          b[1] = lds128<192>(x);
-          Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+    FewReader<STAGE, Tile::TEAMS> r(&sh.bars, ring, p.stages, team);
+    bool ok = true;
+    int item = lo / steps, i = lo + team;              // i: this team's next step
+    for (int from = lo; from < hi; ++item) {
+      const int first = item * steps, to = min(hi, first + steps);
+      const bool whole = from == first;
+      for (; i < to; i += Tile::TEAMS) {
+        if (ok && (ok = r.wait(p.status))) {
+          const int c = (i - first) * Tile::CHUNKS;
+          const uint32_t x = xt + c * 128;
+          uint4 b[2] = {lds128<0>(x), lds128<64>(x)};
+          Tile::mma(acc, r.data + place, r.data + scales, b);
+          if (Tile::CHUNKS == 2 && c + 1 < chunks) {
+            b[0] = lds128<128>(x);
+            b[1] = lds128<192>(x);
+            Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+          }
+          r.release(lane, acc);
         }
+        r.next();
       }
-      r.next();
-      c += Tile::CHUNKS;
-      if (c < chunks && i + 1 < hi) continue;
       // The item's part in this range is done: the second team's sums go to the first, which finishes the item, leaves a part of it to the CTA that began it, or
       // keeps what it has until the others' parts are there.  Two buffers: a team is at most one item ahead of the other.
       float4* mine_ = sh.teams[item & 1][warp & 3];
@@ -588,7 +588,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
         }
         if (!whole) {
           for (int m = 0; m < 2; ++m) p.parts[((blockIdx.x * 4 + warp) * 2 + m) * 32 + lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
-        } else if (c >= chunks) {
+        } else if (to == first + steps) {
           finish(item0 + item, acc);
         } else {
           for (int m = 0; m < 2; ++m) for (int j = 0; j < 4; ++j) left[m][j] = acc[m][j];
@@ -596,9 +596,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[0][j] = acc[1][j] = 0.f;
-      c = 0;
-      whole = true;
-      ++item;
+      from = to;
     }
   }
   __syncwarp();
@@ -686,35 +684,34 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
     if (!ok) r.drain(bars);
   } else {
     float acc[2][4] = {};
-    FewReader<STAGE> r(&bars, ring, STAGES);
+    FewReader<STAGE, TEAMS> r(&bars, ring, STAGES, team);
     const uint32_t place = Tile::place(r0, g, q), scales = Tile::scales(r0), hs = H_OFF + g * H_LD + q * 16;
-    uint32_t meets = lo < hi && plan.slot[d][g] != 255 ? ~0u : 0u;     // else what lies in the token's place is left over
     auto masked = [](const uint4& v, uint32_t m) { return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m); };
-    int turn = 0;
-    for (int i = lo; i < hi; ++i) {
-      r.release(lane);
-      if (turn == team && ok && (ok = r.wait(p.status))) {
-        const uint32_t x = r.data + hs;
-        uint4 b[2] = {masked(lds128<0>(x), meets), masked(lds128<64>(x), meets)};
-        Tile::mma(acc, r.data + place, r.data + scales, b);
-        if (c + 1 < chunks) {
-          b[0] = masked(lds128<128>(x), meets);
-          b[1] = masked(lds128<192>(x), meets);
-          Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+    int i = lo + team;                                   // this team's next step
+    for (int from = lo; from < hi; ++d) {
+      const int begin = d * steps, to = min(hi, begin + steps);
+      const uint32_t meets = plan.slot[d][g] != 255 ? ~0u : 0u;        // else what lies in the token's place is left over
+      for (; i < to; i += TEAMS) {
+        if (ok && (ok = r.wait(p.status))) {
+          const uint32_t x = r.data + hs;
+          uint4 b[2] = {masked(lds128<0>(x), meets), masked(lds128<64>(x), meets)};
+          Tile::mma(acc, r.data + place, r.data + scales, b);
+          if ((i - begin) * Tile::CHUNKS + 1 < chunks) {
+            b[0] = masked(lds128<128>(x), meets);
+            b[1] = masked(lds128<192>(x), meets);
+            Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+          }
+          r.release(lane, acc);
         }
+        r.next();
       }
-      turn = turn + 1 == TEAMS ? 0 : turn + 1;
-      r.next();
-      c += Tile::CHUNKS;
-      if (c < chunks && i + 1 < hi) continue;
       // an expert's part is done: it counts for the tokens that meet it (weights that are not numbers stay with them)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (plan.slot[d][q * 2 + (j & 1)] != 255) { sum[0][j] += acc[0][j]; sum[1][j] += acc[1][j]; }
         acc[0][j] = acc[1][j] = 0.f;
       }
-      c = 0;
-      if (++d < plan.met) meets = plan.slot[d][g] != 255 ? ~0u : 0u;
+      from = to;
     }
   }
   __syncwarp();
