@@ -28,8 +28,8 @@ template <int N> struct Int { static constexpr int value = N; };
 enum FewWeights : int { FEW_BF16 = 0, FEW_FP4_F16 = 1, FEW_FP4_BF16 = 2 };   // packed: the records of gemm_fp4.cu in their two forms
 constexpr int FEW_TOKENS = 8, FEW_TOP = 32, FEW_EXPERTS = 1024, FEW_MET = FEW_TOKENS * FEW_TOP;
 constexpr int FEW_CLUSTER = 8;
-constexpr int FEW_THREADS = 288, FEW_STAGES = 16;
-constexpr size_t FEW_SMEM_TWO = 112 * 1024, FEW_SMEM_ONE = 227 * 1024;          // shared memory of a CTA, with two or one on an SM
+constexpr int FEW_THREADS = 288, FEW_DOWN_THREADS = 320, FEW_STAGES = 16;
+constexpr size_t FEW_SMEM_TWO = 113 * 1024, FEW_SMEM_ONE = 227 * 1024;          // shared memory of a CTA, with two or one on an SM
 constexpr int FEW_DOWN_ROWS = 64, FEW_DOWN_RING = 96 * 1024, FEW_OUT = FEW_DOWN_ROWS * FEW_TOKENS;
 constexpr int FEW_MAX_CTAS = 320;                                               // of the first kernel: partial sums of a cut item, 4 KB each
 constexpr long long FEW_PREFETCH = 40 << 20;
@@ -37,9 +37,9 @@ constexpr long long FEW_PREFETCH = 40 << 20;
 // What the first kernel leaves for the second.
 struct alignas(16) FewPlan {
   int met, unused[3];                       // experts that any token meets, in ascending order
-  int expert[FEW_MET];
+  uint16_t expert[FEW_MET];
   uint8_t slot[FEW_MET][FEW_TOKENS];        // which choice of the token the expert is; 255: none
-  int ids[FEW_TOKENS * FEW_TOP];            // [token][choice]
+  uint16_t ids[FEW_TOKENS * FEW_TOP];       // [token][choice]
   float share[FEW_TOKENS * FEW_TOP];
 };
 static_assert(sizeof(FewPlan) % 16 == 0, "h follows the plan");
@@ -59,7 +59,7 @@ struct FewArgs {
   FewPlan* plan;
   float4* parts;        // [CTA][warp][lane] sums of the first kernel's cut items
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
-  int stages, splits;   // of the first kernel's ring; CTAs of a cluster of the second
+  int stages, ring_bytes, splits;   // of the first kernel's ring, and its room; CTAs of a cluster of the second
   int* status;
 };
 
@@ -104,6 +104,9 @@ template <int OFF> __device__ __forceinline__ uint32_t lds8(uint32_t at) {
   asm volatile("ld.shared.u8 %0, [%1+%2];" : "=r"(v) : "r"(at), "n"(OFF));
   return v;
 }
+
+// A thread's arrival on a barrier when its copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 
 // A stage of the ring holds CHUNKS steps of 64 k values of a tile of ROWS weight rows, as they lie in memory: packed records (codes, then scales), or (bf16) a
 // box of 64 columns with the 128-byte swizzle.  A warp multiplies 16 of the rows: row r0 of the tile (lanes 4 g .. 4 g + 3) and row r1.
@@ -179,7 +182,9 @@ struct FewTile {
       half(Int<1>{}, Int<1>{});
     }
   }
-  // Copies n steps from `chunk` on of rows row .. row + ROWS - 1 of expert e to a stage, counted in bytes on its barrier; by one thread.
+  // Copies n steps from `chunk` on of rows row .. row + ROWS - 1 of expert e to a stage, counted in bytes on its barrier; by one thread.  Of half a
+  // record's rows: their codes ..
+  static constexpr int COPIED = W == FEW_BF16 || ROWS == 128 ? BYTES : ROWS * 32;
   static __device__ __forceinline__ void copy(uint8_t* dst, uint64_t* bar, const CUtensorMap* map, const void* packed, int e, int row, int chunk, int n, int N, int K) {
     if constexpr (W == FEW_BF16) {
       for (int j = 0; j < n; ++j) tma_load_2d(dst + j * BYTES, map, bar, (chunk + j) * 64, e * N + row);
@@ -191,10 +196,17 @@ struct FewTile {
           bulk_copy_g2s(dst + j * BYTES, rec, FP4_RECORD_BYTES, bar);
         } else {
           bulk_copy_g2s(dst + j * BYTES, rec + (row & 127) * 32, ROWS * 32, bar);
-          bulk_copy_g2s(dst + j * BYTES + ROWS * 32, rec + 128 * 32 + (row & 127) * 2, ROWS * 2, bar);
         }
       }
     }
+  }
+  // .. and the scales of half a record's rows, by a warp in pieces of 16 bytes
+  static __device__ __forceinline__ void copy_scales(uint8_t* dst, const void* packed, int e, int row, int chunk, int n, int N, int K, int lane) {
+    static_assert(W == FEW_BF16 || ROWS * 2 % 16 == 0, "pieces");
+    constexpr int EACH = ROWS * 2 / 16;
+    const int tiles = (N + 127) >> 7, j = lane / EACH;
+    const uint8_t* rec = static_cast<const uint8_t*>(packed) + (((long long)e * (K >> 6) + chunk + j) * tiles + (row >> 7)) * FP4_RECORD_BYTES;
+    if (j < n) cp_async16(dst + j * BYTES + ROWS * 32 + lane % EACH * 16, rec + 128 * 32 + (row & 127) * 2 + lane % EACH * 16, true);
   }
 };
 
@@ -210,8 +222,8 @@ __device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // 
 // ------------------------------------------------------------------------------- ring of copies
 // Warp 8 copies, warps 0 .. 7 multiply.  All waits are bounded; after a failed one every warp leaves its loop.
 struct FewBars { uint64_t full[FEW_STAGES], empty[FEW_STAGES]; int abort; };
-__device__ __forceinline__ void few_init(FewBars& b, int stages, int warps) {      // warps that read a stage
-  for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], 1); mbar_init(&b.empty[s], warps); }
+__device__ __forceinline__ void few_init(FewBars& b, int stages, int writers, int warps) {      // warps that copy to a stage, and that read it
+  for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], writers); mbar_init(&b.empty[s], warps); }
   b.abort = 0;
   mbar_fence_init();
 }
@@ -272,13 +284,16 @@ struct FewReader {                     // the multiplying side: every TEAMS-th s
 };
 
 // ------------------------------------------------------------------------------- router, choice
-// Shared memory of the first kernel.
+// Shared memory of the first kernel: what stands where the ring comes, until the experts are chosen (then logits [T][E]) ..
+struct FewBefore {
+  float red[FEW_THREADS / 32][16 * FEW_TOKENS];
+  uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
+};
+// .. and behind the ring
 struct FewShared {
   FewBars bars;
   float4 teams[2][4][64];             // [item][warp][half of its rows, lane] sums of the second team
-  float red[FEW_THREADS / 32][16 * FEW_TOKENS];
   uint32_t top[FEW_TOKENS];          // bits of the rows' largest magnitudes
-  uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
   FewPlan plan;
 };
 static_assert(sizeof(FewShared) % 16 == 0, "16-byte accesses to what follows");
@@ -342,16 +357,17 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  FewShared& sh = *reinterpret_cast<FewShared*>(ring + p.stages * STAGE);
-  float* logits = reinterpret_cast<float*>(&sh + 1);                                         // [T][E]
+  FewBefore& pre = *reinterpret_cast<FewBefore*>(ring);
+  float* logits = reinterpret_cast<float*>(&pre + 1);                                        // [T][E]
+  FewShared& sh = *reinterpret_cast<FewShared*>(ring + p.ring_bytes);
   const int Hp = (p.H + 63) / 64 * 64, xs_ld = Hp + 32;              // 16-bit values a row: neighbours start 64 bytes apart in the banks
-  uint16_t* xs = reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(logits) + (size_t(p.T) * p.E * 4 + 15) / 16 * 16);
+  uint16_t* xs = reinterpret_cast<uint16_t*>(&sh + 1);
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = int(cluster_ctarank());
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the others' shared memory is written only once they run
-  for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) sh.mask[e] = 0;
+  for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) pre.mask[e] = 0;
   if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
-  if (threadIdx.x == 0) few_init(sh.bars, p.stages, 8 / Tile::TEAMS);
+  if (threadIdx.x == 0) few_init(sh.bars, p.stages, 1, 8 / Tile::TEAMS);
   __syncwarp();
   __syncthreads();
 
@@ -390,15 +406,24 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const __nv_bfloat16* w0 = p.router + (long long)(r0 ? e0 + g : 0) * p.H;
     const __nv_bfloat16* w1 = p.router + (long long)(r1 ? e0 + g + 8 : 0) * p.H;
+    auto fetch = [&](const __nv_bfloat16* at, bool there) { return there ? *reinterpret_cast<const uint4*>(at) : zero; };
+    if (e0 + 8 < e_end) {
 #pragma unroll 5
-    for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += FEW_THREADS) {
-      const bool in = k < p.H;
-      const uint4 a0 = r0 && in ? *reinterpret_cast<const uint4*>(w0 + k) : zero, a1 = r1 && in ? *reinterpret_cast<const uint4*>(w1 + k) : zero;
-      const uint4 b = g < p.T && in ? *reinterpret_cast<const uint4*>(p.x + g * p.ldx + k) : zero;
-      mma_bf16_32(acc, a0, a1, b);
+      for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += FEW_THREADS) {
+        const bool in = k < p.H;
+        const uint4 a0 = fetch(w0 + k, r0 && in), a1 = fetch(w1 + k, r1 && in), b = fetch(p.x + g * p.ldx + k, g < p.T && in);
+        mma_bf16_32(acc, a0, a1, b);
+      }
+    } else {                                             // (up to eight: more of k on its way at once)
+#pragma unroll 10
+      for (int k = warp * 32 + q * 8; k < (p.H + 31) / 32 * 32; k += FEW_THREADS) {
+        const bool in = k < p.H;
+        const uint4 a0 = fetch(w0 + k, r0 && in), b = fetch(p.x + g * p.ldx + k, g < p.T && in);
+        mma_bf16_32(acc, a0, zero, b);
+      }
     }
-    *reinterpret_cast<float2*>(&sh.red[warp][g * 8 + q * 2]) = make_float2(acc[0][0] + acc[1][0], acc[0][1] + acc[1][1]);
-    *reinterpret_cast<float2*>(&sh.red[warp][(g + 8) * 8 + q * 2]) = make_float2(acc[0][2] + acc[1][2], acc[0][3] + acc[1][3]);
+    *reinterpret_cast<float2*>(&pre.red[warp][g * 8 + q * 2]) = make_float2(acc[0][0] + acc[1][0], acc[0][1] + acc[1][1]);
+    *reinterpret_cast<float2*>(&pre.red[warp][(g + 8) * 8 + q * 2]) = make_float2(acc[0][2] + acc[1][2], acc[0][3] + acc[1][3]);
     __syncthreads();
     if (!met_cluster) { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); met_cluster = true; }
     if (threadIdx.x < 128) {
@@ -406,7 +431,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
       if (e < e_end && t < p.T) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < FEW_THREADS / 32; ++w) v += sh.red[w][threadIdx.x];
+        for (int w = 0; w < FEW_THREADS / 32; ++w) v += pre.red[w][threadIdx.x];
         if (p.router_b) v += bf2f(p.router_b[e]);
         const uint32_t at = smem_u32(logits + t * p.E + e);
 #pragma unroll
@@ -444,29 +469,30 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     else if (p.E <= 256) few_choose<8>(row, p.E, p.top, p.rule, lane, id, share);
     else few_choose<32>(row, p.E, p.top, p.rule, lane, id, share);
     if (lane < p.top) {
-      sh.plan.ids[warp * p.top + lane] = id;
+      sh.plan.ids[warp * p.top + lane] = uint16_t(id);
       sh.plan.share[warp * p.top + lane] = share;
-      atomicOr(&sh.mask[id], 1u << warp);
+      atomicOr(&pre.mask[id], 1u << warp);
     }
   }
   __syncthreads();
   if (warp == 0) {
     int n = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const bool here = e0 + lane < p.E && sh.mask[e0 + lane];
+      const bool here = e0 + lane < p.E && pre.mask[e0 + lane];
       const uint32_t b = __ballot_sync(0xffffffffu, here);
       const int at = n + __popc(b & ((1u << lane) - 1));
       if (here) {
-        sh.plan.expert[at] = e0 + lane;
+        sh.plan.expert[at] = uint16_t(e0 + lane);
         *reinterpret_cast<uint2*>(sh.plan.slot[at]) = make_uint2(0xffffffffu, 0xffffffffu);
-        sh.mask[e0 + lane] = uint32_t(at);         // from here on: the expert's place in the list
+        pre.mask[e0 + lane] = uint32_t(at);         // from here on: the expert's place in the list
       }
       n += __popc(b);
     }
     if (lane == 0) sh.plan.met = n;
     __syncwarp();
-    for (int i = lane; i < p.T * p.top; i += 32) sh.plan.slot[sh.mask[sh.plan.ids[i]]][i / p.top] = uint8_t(i % p.top);
+    for (int i = lane; i < p.T * p.top; i += 32) sh.plan.slot[pre.mask[sh.plan.ids[i]]][i / p.top] = uint8_t(i % p.top);
   }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // copies take the place of what stood in the ring's
   __syncthreads();
   if (blockIdx.x == 0) {
     const uint4* src = reinterpret_cast<const uint4*>(&sh.plan);
@@ -618,7 +644,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
 }
 
 template <int W>
-__global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
+__global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
   using Tile = FewTile<W, FEW_DOWN_ROWS>;
   constexpr int H_LD = Tile::CHUNKS * 128 + 64, H_OFF = Tile::CHUNKS * Tile::BYTES, STAGE = (H_OFF + FEW_TOKENS * H_LD + 1023) / 1024 * 1024;
   constexpr int STAGES = Tile::ring(FEW_DOWN_RING, STAGE), TEAMS = Tile::TEAMS;
@@ -631,11 +657,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = int(cluster_ctarank()), splits = p.splits, n0 = int(blockIdx.x) / splits * FEW_DOWN_ROWS;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (threadIdx.x == 0) few_init(bars, STAGES, 8 / TEAMS);
+  if (threadIdx.x == 0) few_init(bars, STAGES, 1 + 32, 8 / TEAMS);
   pdl_launch_dependents();
   {
     const uint4* src = reinterpret_cast<const uint4*>(p.plan);
-    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_THREADS) reinterpret_cast<uint4*>(&plan)[i] = src[i];
+    for (int i = threadIdx.x; i < int(sizeof(FewPlan) / 16); i += FEW_DOWN_THREADS) reinterpret_cast<uint4*>(&plan)[i] = src[i];
   }
   __syncthreads();
   const int chunks = p.I >> 6, steps = (chunks + Tile::CHUNKS - 1) / Tile::CHUNKS, total = plan.met * steps;
@@ -652,7 +678,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       int n, t;
-      if (output(int(threadIdx.x) + k * FEW_THREADS, n, t))
+      if (output(int(threadIdx.x) + k * FEW_DOWN_THREADS, n, t))
         for (int j = 0; j < p.top; ++j) bias[k] += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
     }
   }
@@ -660,28 +686,60 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
   float sum[2][4] = {};
   const int team = warp >> 1, r0 = (warp & 1) * 32 + g;
   int d = lo / steps, c = (lo - d * steps) * Tile::CHUNKS;
-  if (warp == 8) {
+  if (warp == 8) {                       // weights
     FewRing r{STAGES};
     for (int i = lo; i < hi; ++i) {
       ok = r.wait_empty(bars, p.status);
       if (!ok) break;
       const int n = min(Tile::CHUNKS, chunks - c);
-      uint8_t* st = ring + r.s * STAGE;
-      uint64_t* bar = &bars.full[r.s];
-      const int slot = lane < p.T ? plan.slot[d][lane & 7] : 255;
-      const uint32_t meet = __ballot_sync(0xffffffffu, slot != 255);
       if (elect_one()) {
-        mbar_expect_tx(bar, n * (Tile::BYTES + __popc(meet) * 128));
-        Tile::copy(st, bar, &map, p.down, plan.expert[d], n0, c, n, p.H, p.I);
+        mbar_expect_tx(&bars.full[r.s], n * Tile::COPIED);
+        Tile::copy(ring + r.s * STAGE, &bars.full[r.s], &map, p.down, plan.expert[d], n0, c, n, p.H, p.I);
       }
-      __syncwarp();
-      if (slot != 255) bulk_copy_g2s(st + H_OFF + lane * H_LD, p.h + (long long)(lane * p.top + slot) * p.I + c * 64, n * 128, bar);
       __syncwarp();
       r.next();
       c += Tile::CHUNKS;
       if (c >= chunks) { c = 0; ++d; }
     }
     if (!ok) r.drain(bars);
+  } else if (warp == 9) {                // scales of half records, and the activations of the tokens that meet the expert
+    FewRing r{STAGES};
+    constexpr int PAIRS = FEW_TOKENS / 2;
+    const int piece = lane & 15;                         // a half of the warp takes a token at a time, 16 bytes a lane
+    const uint16_t* from[PAIRS] = {};                    // every second one of the tokens that meet expert `now`: its activations, and its place in a stage
+    int place[PAIRS] = {}, pairs = 0, now = -1;
+    for (int i = lo; i < hi; ++i) {
+      if (d != now) {
+        now = d;
+        uint32_t left = __ballot_sync(0xffffffffu, lane < p.T && plan.slot[d][lane & 7] != 255);
+        pairs = (__popc(left) + 1) / 2;
+        if (lane >= 16) left &= left - 1;
+#pragma unroll
+        for (int u = 0; u < PAIRS; ++u) {
+          const int t = left ? __ffs(left) - 1 : -1;
+          left &= left - 1;
+          left &= left - 1;
+          place[u] = t < 0 ? -1 : H_OFF + t * H_LD + piece * 16;
+          if (t >= 0) from[u] = p.h + (long long)(t * p.top + plan.slot[d][t]) * p.I + piece * 8;
+        }
+      }
+      ok = r.wait_empty(bars, p.status);
+      if (!ok) break;
+      const int n = min(Tile::CHUNKS, chunks - c);
+      uint8_t* st = ring + r.s * STAGE;
+      if constexpr (Tile::COPIED < Tile::BYTES) Tile::copy_scales(st, p.down, plan.expert[d], n0, c, n, p.H, p.I, lane);
+#pragma unroll
+      for (int u = 0; u < PAIRS; ++u) {
+        if (u >= pairs) break;
+        if (place[u] >= 0 && piece < n * 8) cp_async16(st + place[u], from[u] + c * 64, true);
+      }
+      __syncwarp();
+      cp_async_arrive(&bars.full[r.s]);
+      r.next();
+      c += Tile::CHUNKS;
+      if (c >= chunks) { c = 0; ++d; }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     float acc[2][4] = {};
     FewReader<STAGE, TEAMS> r(&bars, ring, STAGES, team);
@@ -730,7 +788,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     int n, t;
-    const int i = int(threadIdx.x) + k * FEW_THREADS;
+    const int i = int(threadIdx.x) + k * FEW_DOWN_THREADS;
     if (!output(i, n, t)) continue;
     float v = 0.f;
     for (int s = 0; s < splits * TEAMS; ++s) v += red[s * per + i];
@@ -739,26 +797,26 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_down_kernel(const __grid_c
 }
 
 // --------------------------------------------------------------------------------- host side
-// Shared memory of the first kernel besides its ring: rows and logits of all tokens
-static size_t few_fixed(int T, int H, int E) {
-  return 1024 + sizeof(FewShared) + (size_t(T) * E * 4 + 15) / 16 * 16 + size_t(T) * ((H + 63) / 64 * 64 + 32) * 2;
-}
-// A place in the ring for each team (of the largest stage) has to be left.
+// Shared memory of the first kernel: besides its ring's, and what its ring has to have room for at least (a place for each team, of the largest stage)
+static size_t few_fixed(int T, int H) { return 1024 + sizeof(FewShared) + size_t(T) * ((H + 63) / 64 * 64 + 32) * 2; }
+static size_t few_before(int T, int E) { return (sizeof(FewBefore) + size_t(T) * E * 4 + 15) / 16 * 16; }
 static bool few_fits(int T, int H, int E) {
   using Tile = FewTile<FEW_BF16, 128>;
+  constexpr size_t least = Tile::TEAMS * Tile::CHUNKS * Tile::BYTES;
   static_assert(Tile::CHUNKS * Tile::BYTES >= FewTile<FEW_FP4_F16, 128>::CHUNKS * FewTile<FEW_FP4_F16, 128>::BYTES, "the largest stage");
-  return H <= 65536 && few_fixed(T, H, E) + Tile::TEAMS * Tile::CHUNKS * Tile::BYTES <= FEW_SMEM_ONE;
+  return H <= 65536 && few_fixed(T, H) + max(least, few_before(T, E)) <= FEW_SMEM_ONE;
 }
 
 template <int W>
 static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
   using Tile = FewTile<W, 128>;
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
-  const size_t fixed = few_fixed(p.T, p.H, p.E);
-  // Two CTAs an SM where that leaves each a ring of 32 KiB: more warps to expand and multiply; else one with what there is.
-  const int two = fixed + 32 * 1024 <= FEW_SMEM_TWO;
+  const size_t fixed = few_fixed(p.T, p.H), before = few_before(p.T, p.E);
+  // Two CTAs an SM where that leaves each a ring of 48 KiB: more warps to expand and multiply; else one with what there is.
+  const int two = fixed + max(size_t(48 * 1024), before) <= FEW_SMEM_TWO;
   const size_t room = two ? FEW_SMEM_TWO : FEW_SMEM_ONE;
   p.stages = Tile::ring(int(room - fixed), STAGE);
+  p.ring_bytes = int(max(size_t(p.stages * STAGE), before));
   CUtensorMap gate_up = {}, down = {};
   if (W == FEW_BF16 && (!encode_map_2d(&gate_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.gate_up, uint64_t(p.E) * 2 * p.I, p.H, uint64_t(p.H) * 2, 128, 64, CU_TENSOR_MAP_SWIZZLE_128B) ||
                         !encode_map_2d(&down, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.down, uint64_t(p.E) * p.H, p.I, uint64_t(p.I) * 2, FEW_DOWN_ROWS, 64, CU_TENSOR_MAP_SWIZZLE_128B)))
@@ -788,12 +846,13 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
     clusters = min(clusters, FEW_MAX_CTAS / FEW_CLUSTER);
     if (tracked) clusters_at[dev][two] = clusters;
   }
-  cfg.dynamicSmemBytes = fixed + p.stages * STAGE;
+  cfg.dynamicSmemBytes = fixed + p.ring_bytes;
   cfg.gridDim = dim3(unsigned(clusters * FEW_CLUSTER));
   if (cudaLaunchKernelEx(&cfg, few_gate_up_kernel<W>, gate_up, p) != cudaSuccess) return -4;
   const int tiles = (p.H + FEW_DOWN_ROWS - 1) / FEW_DOWN_ROWS;
   p.splits = max(1, min(FEW_CLUSTER, 2 * sm_count / tiles));                          // two CTAs an SM
   attr[0].val.clusterDim = {unsigned(p.splits), 1, 1};
+  cfg.blockDim = dim3(FEW_DOWN_THREADS);
   cfg.dynamicSmemBytes = FEW_DOWN_RING + 1024;
   cfg.gridDim = dim3(unsigned(tiles * p.splits));
   return cudaLaunchKernelEx(&cfg, few_down_kernel<W>, down, p) == cudaSuccess ? 0 : -4;
@@ -821,7 +880,7 @@ OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router,
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,
             static_cast<const __nv_bfloat16*>(gate_up_b), down, static_cast<const __nv_bfloat16*>(down_b), static_cast<__nv_bfloat16*>(out), T, H, I, E, top,
             rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<float4*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)),
-            reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL), 0, 0, status};
+            reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL), 0, 0, 0, status};
   if ((long long)E * 2 * I > 0x7fffffff || (long long)E * H > 0x7fffffff || (long long)min(E, T * top) * I * H > 1LL << 37) return -5;   // (32-bit counts of steps)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, sm_count, s);
