@@ -1,16 +1,23 @@
-// A whole mixture-of-experts layer for up to eight tokens in two kernels, bound by the bytes of the experts that the tokens meet.
+// A whole mixture-of-experts layer for up to eight tokens in two kernels, bound by the bytes of the experts that the tokens meet and, with few bytes, by latency.
 //
 // few_gate_up_kernel: every cluster of eight CTAs computes all router logits for itself (an eighth of the experts per CTA, exchanged through distributed
 // shared memory), so that each CTA can choose the experts, list those that any token meets, and go on to their gate and up rows without a kernel or a
-// grid barrier in between; the router is small beside the experts and comes from L2.  A warp computes eight features of one expert for all tokens: the
+// grid barrier in between; the router is small beside the experts and comes from L2.  A warp computes sixteen features of one expert for all tokens: the
 // rows of an `mma.sync` tile of 16 are eight gate rows and the eight up rows of the same features, its columns the tokens, so that a thread holds a
 // gate and its up value and writes share * act(gate, up).  The work of a cluster (items of 64 features, in steps of k) is cut into eight equal ranges; of an
 // item that a range border cuts, the later parts' sums go through memory to the CTA that began it.
-// few_down_kernel: a cluster computes 64 columns of the output; its CTAs, and two teams of warps in each, take equal parts of the sequence (expert, k); their
-// sums are sent to the CTA that finishes an output and added there in a fixed order.
+// few_down_kernel: a cluster computes 64 columns of the output; its CTAs take equal parts of the sequence (expert, k); their sums are sent to the CTA that finishes
+// an output and added there in a fixed order.
+// In both the warps of a CTA form teams that take turns at the stages of a ring and add their sums in a fixed order: more stages are in work at once.
 //
 // `mma.sync` is used on purpose: its eight columns are the eight tokens, and weights go from shared memory to registers in the order in which they lie in
-// memory, with the k index of a product permuted alike for both operands.  A ring of bulk copies per CTA keeps some 100 KB an SM in flight.
+// memory, with the k index of a product permuted alike for both operands.  A ring of bulk copies per CTA keeps 50 to 70 KB in flight, twice an SM.  A bulk copy costs
+// some 30 ns of an SM however small it is, so that what is in small pieces (scales of half a record, a step's activations) is copied by a warp's threads: the down products
+// of 7 tokens in 30 us instead of 40.
+//
+// Measured (us a layer, weights from memory; both kernels take 18 of them with hardly any weights: launches, the router, the choice, the first bytes, the sums):
+// 1 token, 4 of 32 mxfp4 experts of 2880: 28; 7 tokens of the same 88 (2.9 TB/s); 8 tokens, 8 of 128 of 1472: 111 (3.1); 1 token, 8 of 128 bf16 experts of 768: 27;
+// 8 tokens, 2 of 8 bf16 experts of 14336: 450 (5.6).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
 //
 // Roundings: the router's logits, all sums and the activation are fp32.  The activations times routing weights travel between the kernels in 16 bits (the
 // operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16, where values beyond 65504 become that.  The rows meet packed
@@ -57,7 +64,7 @@ struct FewArgs {
   int T, H, I, E, top, rule, act;
   float alpha, limit;
   FewPlan* plan;
-  float4* parts;        // [CTA][warp][lane] sums of the first kernel's cut items
+  float4* parts;        // [CTA][warp][half][lane] sums of the first kernel's cut items
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
   int stages, ring_bytes, splits;   // of the first kernel's ring, and its room; CTAs of a cluster of the second
   int* status;
@@ -109,7 +116,8 @@ template <int OFF> __device__ __forceinline__ uint32_t lds8(uint32_t at) {
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory"); }
 
 // A stage of the ring holds CHUNKS steps of 64 k values of a tile of ROWS weight rows, as they lie in memory: packed records (codes, then scales), or (bf16) a
-// box of 64 columns with the 128-byte swizzle.  A warp multiplies 16 of the rows: row r0 of the tile (lanes 4 g .. 4 g + 3) and row r1.
+// box of 64 columns with the 128-byte swizzle.  A warp multiplies 32 of the rows in two tiles of 16: row r0 of the first (lanes 4 g .. 4 g + 3) and the row APART behind it, and
+// those NEXT behind both.
 template <int W, int ROWS>
 struct FewTile {
   static constexpr int CHUNKS = W == FEW_BF16 && ROWS == 128 ? 1 : 2;
@@ -220,7 +228,7 @@ __device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // 
 }
 
 // ------------------------------------------------------------------------------- ring of copies
-// Warp 8 copies, warps 0 .. 7 multiply.  All waits are bounded; after a failed one every warp leaves its loop.
+// Warps 0 .. 7 multiply, the others copy.  All waits are bounded; after a failed one every warp leaves its loop.
 struct FewBars { uint64_t full[FEW_STAGES], empty[FEW_STAGES]; int abort; };
 __device__ __forceinline__ void few_init(FewBars& b, int stages, int writers, int warps) {      // warps that copy to a stage, and that read it
   for (int s = 0; s < stages; ++s) { mbar_init(&b.full[s], writers); mbar_init(&b.empty[s], warps); }
@@ -812,7 +820,8 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
   using Tile = FewTile<W, 128>;
   constexpr int STAGE = Tile::CHUNKS * Tile::BYTES;
   const size_t fixed = few_fixed(p.T, p.H), before = few_before(p.T, p.E);
-  // Two CTAs an SM where that leaves each a ring of 48 KiB: more warps to expand and multiply; else one with what there is.
+  // Two CTAs an SM where that leaves each a ring of 48 KiB: more warps to multiply, more stages in work (7 mxfp4 tokens of 2880 columns: 98 us, one CTA with 16 stages 123);
+  // else one with what there is (8 bf16 tokens of 4096 columns: 453 us, two with two stages each 497).
   const int two = fixed + max(size_t(48 * 1024), before) <= FEW_SMEM_TWO;
   const size_t room = two ? FEW_SMEM_TWO : FEW_SMEM_ONE;
   p.stages = Tile::ring(int(room - fixed), STAGE);
@@ -824,7 +833,8 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
   static bool configured[OGB_MAX_DEVICES] = {}, configured_down[OGB_MAX_DEVICES] = {};
   if (!set_max_dyn_smem(few_gate_up_kernel<W>, int(FEW_SMEM_ONE), configured) || !set_max_dyn_smem(few_down_kernel<W>, FEW_DOWN_RING + 1024, configured_down)) return -3;
   // Both kernels are launched behind the complete kernels in front of them: CTAs that come in as others leave are placed so that some clusters find no room until the
-  // rest is done (8 tokens of 2 of 8 bf16 experts of 14336 in a row: 913 us a layer with programmatic launches, 590 without).
+  // rest is done (8 tokens of 2 of 8 bf16 experts of 14336 in a row: 913 us a layer with programmatic launches of an earlier form, 590 without; the second kernel's alone: 1 mxfp4 token
+  // 37 to 38 us instead of 31).
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim = {FEW_CLUSTER, 1, 1};

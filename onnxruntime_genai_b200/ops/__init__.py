@@ -385,7 +385,7 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     splits: 0 leaves the kernel to the launcher; n > 0 asks for the one that cuts k in n parts, n < 0 for the one on pairs of SMs with -n token
     tiles where it can take the product (no reduction over ranks, no folded norm).
     w an Fp4Matrix: x (bf16 or fp32 rows, or an Fp4Matrix of the same form) is quantised to 4 bits too, and the block-scaled tensor-core product takes both
-    as they are; splits is not looked at."""
+    as they are; splits is not looked at, and `out` may be the residual, but must not overlap the rows."""
     if isinstance(w, Fp4Matrix):
         if all_reduce or reduce_scatter is not None:
             raise RuntimeError("products of 4-bit floating-point weights are not reduced over ranks")
