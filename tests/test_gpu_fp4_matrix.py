@@ -231,3 +231,37 @@ def test_rows_that_are_not_numbers_or_zero_and_the_product_that_quantises():
             x[1] = 0.0
         got = ops.linear(x, w)
         assert torch.equal(got[0], other) and bool((got[1] == 0).all() if fill == 0.0 else torch.isnan(got[1]).all())
+
+
+def test_no_rows():
+    w, gated = weight(192, 256, "nvfp4"), weight(256, 256, "nvfp4", interleaved=True)
+    x = torch.zeros(0, 256, dtype=torch.bfloat16, device=DEV)
+    for rows in (x, x.float(), ops.quantize_fp4(x)):
+        assert ops.linear(rows, w).shape == (0, 192) and ops.gate_up_act(rows, gated).shape == (0, 128)
+
+
+def test_offsets_beyond_32_bits():
+    """2.2 G numbers: rows of them, weights of them, and the results of 2.2 G."""
+    T, K = 66001, 32768
+    big = torch.empty(T, K, dtype=torch.bfloat16, device=DEV)
+    big.normal_(generator=torch.Generator(DEV).manual_seed(1))
+    q = ops.quantize_fp4(big)
+    last = ops.quantize_fp4(big[-70:])
+    back = q.dequantize(torch.bfloat16)
+    assert torch.equal(back[-70:], last.dequantize(torch.bfloat16)) and torch.equal(back[:3], ops.quantize_fp4(big[:3]).dequantize(torch.bfloat16))
+    del back
+    wq = last.dequantize().double()
+    for rows in (1, 3, 70):                          # as weights
+        x = rows_of("normal", rows, K, torch.bfloat16).to(DEV)
+        xq = ops.quantize_fp4(x).dequantize().double()
+        close(ops.linear(x, q)[:, -70:], xq @ wq.T, xq.abs() @ wq.abs().T, K)
+    del big
+    few = weight(128, K, "nvfp4")                    # as rows
+    wq, xq = few.dequantize().double(), last.dequantize().double()
+    close(ops.linear(q, few)[-70:], xq @ wq.T, xq.abs() @ wq.abs().T, K)
+    del q
+    x, w = rows_of("normal", 16800, 256, torch.bfloat16).to(DEV), weight(128256, 256, "mxfp4")
+    y = ops.linear(x, w)[-5:]
+    xq, wq = ops.quantize_fp4(x[-5:], "mxfp4").dequantize().double(), w.dequantize().double()
+    close(y, xq @ wq.T, xq.abs() @ wq.abs().T, 256)
+    ops.check_kernel_status()

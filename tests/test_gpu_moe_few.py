@@ -147,3 +147,20 @@ def test_refusals_of_device_tensors():
             ops.moe_few_tokens(**{**p, **kw}, top=2)
     with pytest.raises(ValueError, match="different devices"):
         ops.moe_few_tokens(**{**p, "router_b": p["router_b"].cpu()}, top=2)
+
+
+def test_experts_beyond_32_bits():
+    """2.4 G numbers of gate and up weights; the experts behind that border are the ones that are met."""
+    T, E, top, H, I = 3, 256, 2, 4608, 1024
+    g = torch.Generator(DEV).manual_seed(2)
+    n = lambda *s: torch.empty(*s, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    gate_up, down = n(E, 2 * I, H).mul_(H ** -0.5), n(E, H, I).mul_(I ** -0.5)
+    p = dict(x=n(T, H), router_w=torch.zeros(E, H, dtype=torch.bfloat16, device=DEV), router_b=torch.zeros(E, dtype=torch.bfloat16, device=DEV), gate_up_b=None, down_b=None)
+    p["router_b"][250:] = torch.arange(6).to(torch.bfloat16).to(DEV)
+    args = dict(top=top, weights="selected", act="silu", alpha=1.0, limit=0.0)
+    got = ops.moe_few_tokens(gate_up_w=gate_up, down_w=down, **p, **args)
+    last = slice(250, 256)
+    stacked = gate_up[last].view(6, I // 64, 2, 64, H).transpose(1, 2).reshape(6, 2 * I, H)
+    want, tol = exact({**p, "router_w": p["router_w"][last], "router_b": p["router_b"][last]}, dict(gate_up=stacked, gate_up_b=None, down=down[last], down_b=None), **args)
+    assert bool(((got.double() - want).abs() <= tol).all())
+    ops.check_kernel_status()

@@ -166,3 +166,34 @@ def test_model_with_experts_for_few_tokens(precision, tmp_path, monkeypatch):
     replayed = generated(model, prompt, 8)                      # from graphs, four sequences a step
     monkeypatch.setenv("OGB_GENERATOR_GRAPH", "0")
     assert np.array_equal(replayed, generated(model, prompt, 8))
+
+
+def test_engine_with_packed_weights_and_experts(tmp_path, monkeypatch):
+    """Requests of different lengths in one engine: steps of prompts, of a few tokens and of padded batches."""
+    arch = ArchConfig(vocab_size=1024, hidden_size=256, num_layers=2, num_heads=4, num_kv_heads=4, head_dim=64, intermediate_size=128, context_length=256,
+                      bos_token_id=0, eos_token_id=1023, pad_token_id=0, model_type="gptoss", num_experts=8, experts_per_token=2, attn_bias=True, o_bias=True,
+                      mlp_bias=True, attn_sinks=True, sliding_window=16, sliding_layers=[0])
+    d = str(tmp_path)
+    export_model(copy.deepcopy(arch), d, "int4", "cuda", state_dict=random_state_dict(arch, seed=8, std=0.05), linear_format="nvfp4", paged=True, block_size=16,
+                 num_blocks=256, max_batch_size=16)
+    monkeypatch.setenv("OGB_FP4_LINEAR", "1")
+    monkeypatch.setattr(moe, "_FEW", True)
+    model = og.Model(d)
+    engine = og.Engine(model)
+    rng = np.random.RandomState(3)
+    requests = []
+    for n in (5, 70, 1, 9, 33):
+        gp = og.GeneratorParams(model)
+        gp.set_search_options(max_length=n + 12)
+        r = og.Request(gp)
+        r.add_tokens(rng.randint(1, 1000, size=n).astype(np.int32))
+        engine.add_request(r)
+        requests.append(r)
+    seen = {id(r): [] for r in requests}
+    while engine.has_pending_requests():
+        r = engine.step()
+        if r is not None:
+            while r.has_unseen_tokens():
+                seen[id(r)].append(r.get_unseen_token())
+    ops.check_kernel_status()
+    assert all(0 < len(t) <= 12 and all(0 <= v < 1024 for v in t) for t in seen.values())
