@@ -24,9 +24,9 @@ __device__ __forceinline__ void values8(uint32_t codes, float (&v)[8]) {
 // A warp turns a row's k-blocks of 256, eight elements a lane: a block of 16 (32) belongs to two (four) lanes, the codes of a k-block go out as one
 // line of 128 bytes.  `wpr` warps share a row (a power of two up to THREADS / 32) and meet once, at the row's largest value; up to
 // HELD k-blocks a warp stay in registers between the two passes, later ones are read again.
-// With many rows bound by the instructions of a number (some twelve) beside the bytes: 256 threads with eight pieces each, four CTAs an SM (4096 x 14336 bf16 in 36.5 us,
-// 4.1 TB/s; three an SM: 38.8; five with four pieces each, whose rows are partly read twice: 45.8; a CTA that fetches its next row ahead: no gain).  fp32 rows to mxfp4 do
-// not fit 64 registers: three an SM (777 x 2880 in 3.2 us, else 3.8).  Bound by latency with few rows, where twice the warps share a row.
+// With many rows bound by the instructions of a number (some ten) beside the bytes: 256 threads with eight pieces each, four CTAs an SM (4096 x 14336 bf16 in 33.9 us,
+// 4.4 TB/s; when that took 36.5: three an SM 38.8, five with four pieces each, whose rows are partly read twice, 45.8, a CTA that fetches its next row ahead no gain).  fp32
+// rows to mxfp4 do not fit 64 registers: three an SM (777 x 2880 in 3.2 us, else 3.8).  Bound by latency with few rows, where twice the warps share a row.
 constexpr int quantize_ctas(int bytes, int form, int threads) { return threads == 512 ? 2 : bytes == 4 && form == FP4_MX ? 3 : 4; }
 template <typename T, int FORM, bool VEC, int HELD, int THREADS>
 __global__ void __launch_bounds__(THREADS, quantize_ctas(sizeof(T), FORM, THREADS)) quantize_fp4_kernel(const T* __restrict__ x, long long ldx, int K, int wpr, Fp4View out) {

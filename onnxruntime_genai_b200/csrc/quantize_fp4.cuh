@@ -24,6 +24,16 @@ __device__ __forceinline__ uint32_t e4m3_of(float v) {      // 0 <= v <= 448, to
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(v));
   return r & 0xffu;
 }
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(code)));
+  return __half2float(__ushort_as_half(uint16_t(h)));
+}
+__device__ __forceinline__ float reciprocal(float v) {      // within a last place or two, of a normal number
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 // eight numbers to eight codes, the first in the lowest four bits: to nearest, ties to the even code, at most 6
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   uint32_t r;
@@ -96,13 +106,13 @@ __device__ __forceinline__ uint32_t fp4_codes8(const Raw8<T>& r, uint32_t m, flo
       // them), and a quotient by a scale of four bits is a tie or at least 2^-10 away from it, so that rounding it to whole 2^-14, by an addition, puts it right.
       constexpr float grid = 768.f;                                       // 1.5 * 2^9; quotients are at most 9
       code = bad ? 0u : e4m3_of(h);
-      const float inv = code ? __fdividef(1.f, fp4_scale_nv(code)) * over : 0.f;
+      const float inv = code ? reciprocal(e4m3_value(code)) * over : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = __fsub_rn(fmaf(v[i], inv, grid), grid);
     } else {
       // Else: one correction by the exact remainder, with reciprocals that a Newton step makes the nearest ones.
       code = bad ? 0u : e4m3_of(fmaf(fmaf(-h, 6.f, t), sixth, h));
-      const float sc = fp4_scale_nv(code), by = sc * s, near = __fdividef(1.f, sc);
+      const float sc = e4m3_value(code), by = sc * s, near = reciprocal(sc);
       const float inv = code ? fmaf(fmaf(-sc, near, 1.f), near, near) * over : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
