@@ -435,12 +435,15 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     return _gemm(x, w, out, bias, residual, flags, splits, fused)
 
 
+_current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
 def _call_on(index: int, entry: str, *args):
     """Runs an entry point of the kernel library on device `index`, on that device's current stream (the last argument)."""
-    if index != torch._C._cuda_getDevice():
+    if index != _current_device():
         with torch.cuda.device(index):
             return _call_on(index, entry, *args)
-    _lib.check(getattr(_lib.lib(), entry)(*args, torch._C._cuda_getCurrentRawStream(index)), entry)
+    _lib.check(getattr(_lib.lib(), entry)(*args, _current_stream(index)), entry)
 
 
 def quantize_fp4(x, form: str = "nvfp4") -> Fp4Matrix:
@@ -448,16 +451,19 @@ def quantize_fp4(x, form: str = "nvfp4") -> Fp4Matrix:
     "nvfp4": blocks of 16 with an e4m3 scale, a power of two per row; "mxfp4": blocks of 32 with a power of two.  Codes are the nearest ones, ties to the
     even code (csrc/quantize_fp4.cu gives the rules).  A row that holds an infinity or a NaN reads back, and multiplies, as NaN throughout.
     The result serves as the rows of `linear` and `gate_up_act` with weights of the same form, so that several products share one quantisation."""
-    if x.dim() != 2 or x.dtype not in (torch.bfloat16, torch.float32):
+    x32 = x.dtype is torch.float32
+    if x.dim() != 2 or not (x32 or x.dtype is torch.bfloat16):
         raise ValueError(f"quantize_fp4 takes rows [T, K] in bfloat16 or float32, not {tuple(x.shape)} in {x.dtype}")
     T, K = x.shape
     Fp4Matrix.check(T, K, form)
     if not x.is_cuda:
         return fp4_matrix.quantize(x, form)
-    if x.stride(1) != 1:
+    ldx, one = x.stride()
+    if one != 1:
         x = x.contiguous()
+        ldx = K
     data = torch.empty(fp4_matrix.matrix_bytes(T, K, form), dtype=torch.uint8, device=x.device)
-    _call_on(x.get_device(), "ogb_quantize_fp4", x.data_ptr(), x.stride(0), x.dtype == torch.float32, T, K, fp4_matrix.FORMS[form], data.data_ptr())
+    _call_on(x.get_device(), "ogb_quantize_fp4", x.data_ptr(), ldx, x32, T, K, fp4_matrix.FORMS[form], data.data_ptr())
     return Fp4Matrix(data, T, K, form)
 
 
