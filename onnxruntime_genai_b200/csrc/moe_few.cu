@@ -16,8 +16,8 @@
 // of 7 tokens in 30 us instead of 40.
 //
 // Measured (us a layer, weights from memory; both kernels take 18 of them with hardly any weights: launches, the router, the choice, the first bytes, the sums):
-// 1 token, 4 of 32 mxfp4 experts of 2880: 28; 7 tokens of the same 88 (2.9 TB/s); 8 tokens, 8 of 128 of 1472: 111 (3.1); 1 token, 8 of 128 bf16 experts of 768: 27;
-// 8 tokens, 2 of 8 bf16 experts of 14336: 450 (5.6).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
+// 1 token, 4 of 32 mxfp4 experts of 2880: 28; 7 tokens of the same 87 (3.0 TB/s); 8 tokens, 8 of 128 of 1472: 111 (3.2); 1 token, 8 of 128 bf16 experts of 768: 26;
+// 8 tokens, 2 of 8 bf16 experts of 14336: 438 (5.8).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
 //
 // Roundings: the router's logits, all sums and the activation are fp32.  The activations times routing weights travel between the kernels in 16 bits (the
 // operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16, where values beyond 65504 become that.  The rows meet packed
@@ -373,12 +373,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = int(cluster_ctarank());
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the others' shared memory is written only once they run
-  for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) pre.mask[e] = 0;
-  if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
-  if (threadIdx.x == 0) few_init(sh.bars, p.stages, 1, 8 / Tile::TEAMS);
-  __syncwarp();
-  __syncthreads();
-
   // The rows: a warp takes 256 values of a token at a time and keeps the first pieces in registers until the rows' largest magnitudes are known (packed experts:
   // fp16 after a scaling).
   constexpr int HELD = 6, WARPS = FEW_THREADS / 32;
@@ -390,7 +384,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
   uint4 held[HELD];
 #pragma unroll
   for (int h = 0; h < HELD; ++h) held[h] = piece(warp + h * WARPS);
-  if (W == FEW_FP4_F16) {
+  for (int e = threadIdx.x; e < p.E; e += FEW_THREADS) pre.mask[e] = 0;
+  if (threadIdx.x < FEW_TOKENS) sh.top[threadIdx.x] = 0;
+  if (threadIdx.x == 0) few_init(sh.bars, p.stages, 1, 8 / Tile::TEAMS);
+  __syncwarp();
+  __syncthreads();
+
+  auto tops = [&]() {                     // behind the router's loads, so that these are on their way first
     auto largest = [&](int i, const uint4& v) {
       if (i >= pieces) return;
       const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
 #pragma unroll
     for (int h = 0; h < HELD; ++h) largest(warp + h * WARPS, held[h]);
     for (int i = warp + HELD * WARPS; i < pieces; i += WARPS) largest(i, piece(i));
-  }
+  };
 
   // router logits of this CTA's experts: 16 experts x 8 tokens at a time, the warps share k
   const int per = (p.E + FEW_CLUSTER - 1) / FEW_CLUSTER, e_end = min(p.E, (rank + 1) * per);
@@ -430,6 +430,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
         mma_bf16_32(acc, a0, zero, b);
       }
     }
+    if (W == FEW_FP4_F16 && !met_cluster) tops();
     *reinterpret_cast<float2*>(&pre.red[warp][g * 8 + q * 2]) = make_float2(acc[0][0] + acc[1][0], acc[0][1] + acc[1][1]);
     *reinterpret_cast<float2*>(&pre.red[warp][(g + 8) * 8 + q * 2]) = make_float2(acc[0][2] + acc[1][2], acc[0][3] + acc[1][3]);
     __syncthreads();
@@ -665,7 +666,8 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = int(cluster_ctarank()), splits = p.splits, n0 = int(blockIdx.x) / splits * FEW_DOWN_ROWS;
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  if (threadIdx.x == 0) few_init(bars, STAGES, 1 + 32, 8 / TEAMS);
+  if (threadIdx.x == FEW_DOWN_THREADS - 1) few_init(bars, STAGES, 1 + 32, 8 / TEAMS);       // (a thread that has nothing of the plan to fetch)
+  static_assert(sizeof(FewPlan) / 16 < FEW_DOWN_THREADS, "one piece a thread");
   pdl_launch_dependents();
   {
     const uint4* src = reinterpret_cast<const uint4*>(p.plan);
