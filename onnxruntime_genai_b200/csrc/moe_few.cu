@@ -282,12 +282,10 @@ struct FewReader {                     // the multiplying side: every TEAMS-th s
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(full), "r"(ph) : "memory");
     return __all_sync(0xffffffffu, ok) || few_wait_slow(b, full, ph, status);
   }
-  // Hands back the stage.  An arrival does not wait for reads of shared memory that are still on their way (seen as single wrong rows), so it stands behind the sums:
-  // they have been issued then, for which all that was read had to be there.
-  __device__ __forceinline__ void release(int lane, float (&acc)[2][4]) {
-    asm volatile("" : "+f"(acc[0][0]), "+f"(acc[0][1]), "+f"(acc[0][2]), "+f"(acc[0][3]), "+f"(acc[1][0]), "+f"(acc[1][1]), "+f"(acc[1][2]), "+f"(acc[1][3]));
-    __syncwarp();
-    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(full + uint32_t(sizeof(uint64_t)) * FEW_STAGES) : "memory");       // (the stage's `empty`)
+  // Hands back the stage, behind all loads from it: every sum's last product has to have its operands first (in fp16 form rows g and g + 8 have scales of their own).
+  __device__ __forceinline__ void release(int lane, const float (&acc)[2][4]) {
+    const uint32_t read = __float_as_uint(acc[0][0]) | __float_as_uint(acc[0][2]) | __float_as_uint(acc[1][0]) | __float_as_uint(acc[1][2]);
+    mbar_arrive_behind_reads(full + uint32_t(sizeof(uint64_t)) * FEW_STAGES, read, lane);       // (the stage's `empty`)
   }
 };
 

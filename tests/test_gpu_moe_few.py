@@ -164,3 +164,24 @@ def test_experts_beyond_32_bits():
     want, tol = exact({**p, "router_w": p["router_w"][last], "router_b": p["router_b"][last]}, dict(gate_up=stacked, gate_up_b=None, down=down[last], down_b=None), **args)
     assert bool(((got.double() - want).abs() <= tol).all())
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_turns_of_the_rings_repeat(kind):
+    """Stages of both rings are handed back and written again some hundred times a call, beside copies of another stream: always the same result, near the exact one."""
+    T, E, H, I = 8, 4, 1024, 4096
+    p, w = layer(T, E, H, I, kind, False)
+    args = dict(top=2, weights="selected", act="silu", alpha=1.0, limit=0.0)
+    first = ops.moe_few_tokens(**p, **args)
+    want, tol = exact(p, w, **args)
+    assert bool(((first.double() - want).abs() <= tol).all())
+    traffic, side = torch.empty(1 << 27, dtype=torch.uint8, device=DEV), torch.cuda.Stream()
+    differs = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(300):
+        if i % 10 == 0:
+            with torch.cuda.stream(side):
+                traffic[: 1 << 26].copy_(traffic[1 << 26:])
+        differs += (ops.moe_few_tokens(**p, **args) != first).any()
+    torch.cuda.synchronize()
+    assert int(differs) == 0
+    ops.check_kernel_status()
