@@ -91,9 +91,9 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // Hands back what a warp has read from shared memory by plain loads: one arrival (of lane 0) at the barrier with shared address `bar`, for the whole warp.  `read`:
 // of each lane, values that it read or results of them, all that depend on the last loads.  An arrival does not wait for loads whose values are used later, and
 // what a copy then writes over them is the asynchronous proxy's; so the arrival's address is made from a vote over every lane's `read`, and cannot be had before
-// these have come back.  (The vote is always 0: grids of callers have one layer, which the compiler cannot know.)  It also brings the warp together.
-__device__ __forceinline__ void mbar_arrive_behind_reads(uint32_t bar, uint32_t read, int lane) {
-  const uint32_t never = __any_sync(0xffffffffu, (read & blockIdx.z) != 0u) ? 8u : 0u;
+// these have come back.  zero: a number that is 0, which the compiler cannot know, so that the vote is.  It also brings the warp together.
+__device__ __forceinline__ void mbar_arrive_behind_reads(uint32_t bar, uint32_t read, uint32_t zero, int lane) {
+  const uint32_t never = __any_sync(0xffffffffu, (read & zero) != 0u) ? 8u : 0u;
   if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar + never) : "memory");
 }
 __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {

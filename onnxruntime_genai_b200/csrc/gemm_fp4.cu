@@ -364,7 +364,7 @@ fp4_stream_grouped_kernel(const void* __restrict__ A_, int lda, const int* __res
       if (!ok) break;
       const int nk = min(2, num_kb - 2 * pr);
       uint2 ca[2], cb[2];
-      uint32_t ma[2], mb[2];
+      uint32_t ma[2], mb[2], read = 0;
       uint4 x0[2], x1[2];
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
@@ -376,11 +376,11 @@ fp4_stream_grouped_kernel(const void* __restrict__ A_, int lda, const int* __res
           mb[r] = *reinterpret_cast<const uint16_t*>(rec + soff + 16);
           x0[r] = *reinterpret_cast<const uint4*>(xrow + (2 * pr + r) * 128);        // block 0
           x1[r] = *reinterpret_cast<const uint4*>(xrow + (2 * pr + r) * 128 + 64);   // block 1
+          read |= ca[r].x | cb[r].x | ma[r] | mb[r];
         }
       }
-      // the records' bytes are in registers: hand the stage back before the arithmetic
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[s]);
+      // the records' bytes are in registers (a word of every read says so): hand the stage back before the arithmetic
+      mbar_arrive_behind_reads(smem_u32(&empty[s]), read, blockIdx.z, lane);      // (the grid has one layer)
       if (++s == FP4_STREAM_STAGES) { s = 0; phase ^= 1; }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {

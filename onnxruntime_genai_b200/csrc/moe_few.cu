@@ -285,7 +285,7 @@ struct FewReader {                     // the multiplying side: every TEAMS-th s
   // Hands back the stage, behind all loads from it: every sum's last product has to have its operands first (in fp16 form rows g and g + 8 have scales of their own).
   __device__ __forceinline__ void release(int lane, const float (&acc)[2][4]) {
     const uint32_t read = __float_as_uint(acc[0][0]) | __float_as_uint(acc[0][2]) | __float_as_uint(acc[1][0]) | __float_as_uint(acc[1][2]);
-    mbar_arrive_behind_reads(full + uint32_t(sizeof(uint64_t)) * FEW_STAGES, read, lane);       // (the stage's `empty`)
+    mbar_arrive_behind_reads(full + uint32_t(sizeof(uint64_t)) * FEW_STAGES, read, blockIdx.z, lane);       // (the stage's `empty`; grids have one layer)
   }
 };
 

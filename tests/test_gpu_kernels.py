@@ -1217,3 +1217,36 @@ def test_gated_delta_rule_kernel(Hk, Hv, dk, dv):
     _close(state, want_state, rtol=1e-3, atol=1e-3)
     assert torch.equal(state[1].cpu(), want_state[1]) and torch.equal(state[3].cpu(), want_state[3])     # untouched slots
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("T", [1, 7, 14])
+def test_streamed_fp4_experts_repeat(T):
+    """Packed experts in fp16 form on the streaming kernel, whose ring holds twelve k-blocks: 42 of them, in one pass over the rows and in two, beside copies of another
+    stream.  Always the same result, within what the roundings allow of the one in 64 bits."""
+    E, N, K, top = 4, 256, 2688, 2
+    g = torch.Generator().manual_seed(T)
+    codes = torch.randint(0, 16, (E, N, K), dtype=torch.uint8, generator=g)
+    w = ops.Fp4Experts.from_codes(codes, torch.randint(117, 122, (E, N, K // 32), dtype=torch.uint8, generator=g), DEV, half=True)
+    x = torch.randn(T, K, generator=g).to(torch.bfloat16).to(DEV)
+    logits = torch.randn(T, E, generator=g)
+    logits[:, 1] += 10.0                                                   # all tokens meet expert 1: 14 of them are two passes
+    plan = ops.moe_route(logits.to(DEV), top, 0, (0, E), 16)
+    call = lambda: ops.moe_gemm(ops.gather_rows(x, plan.sorted_token, f16=True), w, plan)
+    first = call()
+    rows = x[plan.sorted_token.long()].double()
+    expert = torch.searchsorted(plan.expert_offsets[1:], torch.arange(T * top, dtype=torch.int32, device=DEV), right=True)
+    dense = w.dequantize().double().to(DEV)[expert]
+    want, size = torch.einsum("rk,rnk->rn", rows, dense), torch.einsum("rk,rnk->rn", rows.abs(), dense.abs())
+    # fp32 sums of K products; rows in fp16: exact, but for numbers below its normal ones (half a step of 2^-24); the result in bf16
+    tol = K * 2.0 ** -24 * size + 2.0 ** -25 * dense.abs().sum(-1) + 2.0 ** -8 * want.abs()
+    assert bool(((first.double() - want).abs() <= tol).all())
+    traffic, side = torch.empty(1 << 27, dtype=torch.uint8, device=DEV), torch.cuda.Stream()
+    differs = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(300):
+        if i % 10 == 0:
+            with torch.cuda.stream(side):
+                traffic[: 1 << 26].copy_(traffic[1 << 26:])
+        differs += (call() != first).any()
+    torch.cuda.synchronize()
+    assert int(differs) == 0
+    ops.check_kernel_status()
