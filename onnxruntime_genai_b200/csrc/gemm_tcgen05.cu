@@ -228,7 +228,8 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     for (int k = 0; k < PER; ++k) acc[k] = 0.f;
     for (int i = 0; i < num_st; ++i) {
       const int s = i % STAGES;
-      if (!mbar_wait_bounded(&full_bar[s], (i / STAGES) & 1, abort_flag)) { fail(OGB_ERR_WAIT_TMA); break; }
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_bar[s], (i / STAGES) & 1, abort_flag))) { fail(OGB_ERR_WAIT_TMA); break; }   // the warp gives up as one
+      uint32_t read = 0;                                             // a word of every load
 #pragma unroll
       for (int h = 0; h < KB; ++h) {
         if (h >= blocks_of(i)) break;
@@ -239,12 +240,12 @@ gemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
           if (c < CHUNKS) {
             const uint4 q = *reinterpret_cast<const uint4*>(tile + c * 16);
             const float2 a = unpack_bf16x2(q.x), b = unpack_bf16x2(q.y), cc = unpack_bf16x2(q.z), d = unpack_bf16x2(q.w);
+            read |= q.x;
             acc[k] += a.x * a.x + a.y * a.y + b.x * b.x + b.y * b.y + cc.x * cc.x + cc.y * cc.y + d.x * d.x + d.y * d.y;
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty_bar[s]);
+      mbar_arrive_behind_reads(smem_u32(&empty_bar[s]), read, uint32_t(p.M) >> 31, lane);      // (a count of rows has no sign)
     }
 #pragma unroll
     for (int k = 0; k < PER; ++k) {

@@ -1250,3 +1250,27 @@ def test_streamed_fp4_experts_repeat(T):
     torch.cuda.synchronize()
     assert int(differs) == 0
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("T", [1, 16, 33, 128])
+def test_folded_norm_repeats(T):
+    """A product with its rows' norm folded in, over many more stages than the ring holds, beside copies of another stream: the sums of squares that the idle warps read
+    from the stages are the same every time."""
+    N, K = 384, 16384
+    x, w = _rand(T, K, seed=T), _rand(N, K, std=K ** -0.5, seed=2)
+    first = ops.linear(x, w, norm_eps=1e-5, out_fp32=True)
+    xd, wd = x.double(), w.double()
+    scale = torch.rsqrt((xd * xd).mean(-1, keepdim=True) + 1e-5)
+    # fp32 sums of K products, and of K squares under a square root; a few steps for scale and reciprocal root (whose approximation is two last places off)
+    tol = (K * 2.0 ** -24 * xd.abs() @ wd.abs().T + (K * 2.0 ** -25 + 2.0 ** -21) * (xd @ wd.T).abs()) * scale
+    assert bool(((first.double() - xd @ wd.T * scale).abs() <= tol).all())
+    traffic, side = torch.empty(1 << 27, dtype=torch.uint8, device=DEV), torch.cuda.Stream()
+    differs = torch.zeros((), dtype=torch.int64, device=DEV)
+    for i in range(200):
+        if i % 10 == 0:
+            with torch.cuda.stream(side):
+                traffic[: 1 << 26].copy_(traffic[1 << 26:])
+        differs += (ops.linear(x, w, norm_eps=1e-5, out_fp32=True) != first).any()
+    torch.cuda.synchronize()
+    assert int(differs) == 0
+    ops.check_kernel_status()
