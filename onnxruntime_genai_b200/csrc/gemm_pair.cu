@@ -392,19 +392,23 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           if (g % Cfg::TEAMS != team) continue;
           const int ws = g % WS, kb = i * PAIR_KB + half, rs = g % RAW;
           uint4 out[8];
+          uint32_t read = 0;                                                   // a word of every load
           ok = mbar_wait_bounded(&raw_full[rs], (g / RAW) & 1, abort_flag);
           if (kb < num_kb) {
             const uint8_t* rec = smem + Cfg::RAW_OFF + (rs * PAIR_KB + half) * Cfg::REC_BYTES;
             const uint4 q0 = *reinterpret_cast<const uint4*>(rec + row * 32);
             const uint4 q1 = *reinterpret_cast<const uint4*>(rec + row * 32 + 16);
             const uint32_t words[8] = {q0.x, q0.y, q0.z, q0.w, q1.x, q1.y, q1.z, q1.w};
+            read = q0.x | q1.x;
             if constexpr (FMT == PAIR_W4) {
               const uint2 sz = *reinterpret_cast<const uint2*>(rec + GEMM_BLOCK_N * 32 + row * 8);
+              read |= sz.x;
               const W4Scale sc[2] = {w4_scale(sz.x), w4_scale(sz.y)};
 #pragma unroll
               for (int q = 0; q < 8; ++q) out[q] = deq_w4_word(words[q], sc[q >> 2]);
             } else {
               const uint32_t mul = *reinterpret_cast<const uint16_t*>(rec + GEMM_BLOCK_N * 32 + row * 2);   // exponent fields of the two multipliers
+              read |= mul;
               if constexpr (FMT == PAIR_FP4_F16) {
                 // word (q, b) of the record expands to the 16-byte chunk 4 b + q; the stored byte is code + 6, the fp16 field of 2^(code - 127) is code - 112
                 const uint32_t s0 = ((mul & 0xFFu) - 118u) * 0x04000400u, s1 = ((mul >> 8) - 118u) * 0x04000400u;
@@ -419,7 +423,7 @@ gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
           if (ok && g >= WS) ok = cluster_wait_bounded(&w_empty[ws], ((g / WS) & 1) ^ 1, abort_flag);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) { fail(OGB_ERR_WAIT_TMA); break; }                          // the warp gives up as one
-          if (lane == 0) mbar_arrive(&raw_empty[rs]);                          // every lane has read its row: the vote above
+          mbar_arrive_behind_reads(smem_u32(&raw_empty[rs]), read, blockIdx.z, lane);       // (the grid has one layer)
           if (kb < num_kb) {
             uint8_t* dst = stage_w(ws) + half * W_TILE_BYTES + row * 128;
 #pragma unroll

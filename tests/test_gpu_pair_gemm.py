@@ -184,3 +184,32 @@ def test_pair_activation_of_every_column(act):
     # the sums within k * 2^-23 of their magnitudes (below 60), slopes of at most 1.2 (squares: 2 * 30), fast exponentials and tanh within 2^-11 of half an argument below 8 (beyond, they saturate)
     assert ((out.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + k * 2.0 ** -23 * 60 * (60 if act == "relu2" else 1.2) + 2e-3).all()
     assert (wide[:, :3] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["int4", "mxfp4"])
+def test_expanded_weights_repeat(kind):
+    """Packed weights over many more records than the ring holds, beside copies of another stream: the same result every time."""
+    g = torch.Generator().manual_seed(3)
+    m, n, k = 300, 512, 8192
+    x = _rows(m, k, 9)
+    if kind == "int4":
+        w = W4Weight.from_quantized(torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8), (torch.rand(n, k // 32, generator=g) * 0.01 + 0.001).half(),
+                                    torch.randint(0, 16, (n, k // 32), generator=g, dtype=torch.uint8), "cuda")
+        call = lambda: ops.linear(x, w, splits=-2)
+    else:
+        w = Fp4Experts.from_codes(torch.randint(0, 16, (2, n, k), dtype=torch.uint8, generator=g), torch.randint(117, 122, (2, n, k // 32), dtype=torch.uint8, generator=g), "cuda",
+                                  half=True)
+        plan = ops.moe_route(torch.randn(m, 2, generator=g).cuda(), 1, 0, (0, 2), 0)
+        rows = ops.gather_rows(x, plan.sorted_token, f16=True)
+        call = lambda: ops.moe_gemm(rows, w, plan)
+    first = call()
+    traffic, side = torch.empty(1 << 27, dtype=torch.uint8, device="cuda"), torch.cuda.Stream()
+    differs = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(200):
+        if i % 10 == 0:
+            with torch.cuda.stream(side):
+                traffic[: 1 << 26].copy_(traffic[1 << 26:])
+        differs += (call() != first).any()
+    torch.cuda.synchronize()
+    assert int(differs) == 0
+    ops.check_kernel_status()
