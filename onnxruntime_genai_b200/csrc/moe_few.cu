@@ -20,8 +20,9 @@
 // 8 tokens, 2 of 8 bf16 experts of 14336: 438 (5.8).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
 //
 // Roundings: the router's logits, all sums and the activation are fp32.  The activations times routing weights travel between the kernels in 16 bits (the
-// operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16, where values beyond 65504 become that.  The rows meet packed
-// experts of that form as fp16 after a scaling by a power of two per token, which loses nothing within 2^-38 of a row's largest value.
+// operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16 after a scaling by a power of two per token, expert and 64 features
+// (an item of the first product and a step of the second), which the second product's sums undo: eleven bits down to 2^-28 of the largest of the 64, whatever its size.
+// The rows meet packed experts of that form as fp16 after a scaling by a power of two per token, which loses nothing within 2^-38 of a row's largest value.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -66,6 +67,7 @@ struct FewArgs {
   FewPlan* plan;
   float4* parts;        // [CTA][warp][half][lane] sums of the first kernel's cut items
   uint16_t* h;          // [T * top, I], in groups of eight as the second product reads them
+  float* h_scale;       // [met expert, I / 64, token], fp16 form: what the second product's sums over 64 features are multiplied by
   int stages, ring_bytes, splits;   // of the first kernel's ring, and its room; CTAs of a cluster of the second
   int* status;
 };
@@ -131,8 +133,10 @@ struct FewTile {
   // a lane's place in a step: its part of row r0, and (packed) its scales
   static __device__ __forceinline__ uint32_t place(int r0, int g, int q) { return W == FEW_BF16 ? r0 * 128 + ((q ^ g) << 4) : r0 * 32 + q * (W == FEW_FP4_F16 ? 8 : 4); }
   static __device__ __forceinline__ uint32_t scales(int r0) { return ROWS * 32 + r0 * 2; }
-  // A step: every load, then every product.  at, sc: addresses of the lane's place and scales in it; b: the tokens' values
-  static __device__ __forceinline__ void mma(float (&acc)[2][4], uint32_t at, uint32_t sc, const uint4 (&b)[2]) {
+  // A step: every load, then every product.  at, sc: addresses of the lane's place and scales in it; b: the tokens' values; by (fp16 form, where the tokens' values are
+  // scaled step by step): what the sums of the lane's two tokens are multiplied by
+  template <bool SCALED = false>
+  static __device__ __forceinline__ void mma(float (&acc)[2][4], uint32_t at, uint32_t sc, const uint4 (&b)[2], float2 by = make_float2(1.f, 1.f)) {
     if constexpr (W == FEW_BF16) {
       uint4 a[2][2][2];                                                            // [tile of 16][half of the step][row]
       const uint32_t x = at ^ 64u;                                                 // places 4 and more of a row's eight: (q + 4) ^ g
@@ -167,15 +171,22 @@ struct FewTile {
           few_mma_f16(t[m][i], u[2], v[2], u[3], v[3], b[i].z, b[i].w);
         }
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m) {
+        float z[4] = {};
+        float (&to)[4] = SCALED ? z : acc[m];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float x0 = __uint_as_float(f[m][0][i] << 23), x1 = __uint_as_float(f[m][1][i] << 23);
-          acc[m][0] = fmaf(t[m][i][0], x0, acc[m][0]);
-          acc[m][1] = fmaf(t[m][i][1], x0, acc[m][1]);
-          acc[m][2] = fmaf(t[m][i][2], x1, acc[m][2]);
-          acc[m][3] = fmaf(t[m][i][3], x1, acc[m][3]);
+          to[0] = fmaf(t[m][i][0], x0, to[0]);
+          to[1] = fmaf(t[m][i][1], x0, to[1]);
+          to[2] = fmaf(t[m][i][2], x1, to[2]);
+          to[3] = fmaf(t[m][i][3], x1, to[3]);
         }
+        if constexpr (SCALED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[m][j] = fmaf(z[j], j & 1 ? by.y : by.x, acc[m][j]);
+        }
+      }
     } else {
       auto half = [&](auto i, auto m) {
         constexpr int I_ = decltype(i)::value, R = decltype(m)::value * NEXT;
@@ -208,24 +219,15 @@ struct FewTile {
       }
     }
   }
-  // .. and the scales of half a record's rows, by a warp in pieces of 16 bytes
-  static __device__ __forceinline__ void copy_scales(uint8_t* dst, const void* packed, int e, int row, int chunk, int n, int N, int K, int lane) {
-    static_assert(W == FEW_BF16 || ROWS * 2 % 16 == 0, "pieces");
-    constexpr int EACH = ROWS * 2 / 16;
-    const int tiles = (N + 127) >> 7, j = lane / EACH;
-    const uint8_t* rec = static_cast<const uint8_t*>(packed) + (((long long)e * (K >> 6) + chunk + j) * tiles + (row >> 7)) * FP4_RECORD_BYTES;
-    if (j < n) cp_async16(dst + j * BYTES + ROWS * 32 + lane % EACH * 16, rec + 128 * 32 + (row & 127) * 2 + lane % EACH * 16, true);
-  }
+  // .. and the scales of half a record's rows in pieces of 16 bytes, EACH of them a step: where piece i of a record lies, and where it belongs in a step
+  static constexpr int EACH = ROWS * 2 / 16;
+  static __device__ __forceinline__ int scales_in_record(int row, int i) { return 128 * 32 + (row & 127) * 2 + i * 16; }
+  static __device__ __forceinline__ int scales_in_step(int i) { return ROWS * 32 + i * 16; }
 };
 
 // Eight 16-bit values in the order in which a lane's eight weights of a row come out of their load: pairs (0, 1) (2, 3) .. or, from records in fp16 form,
 // (0, 4) (1, 5) (2, 6) (3, 7).
 template <int W> __device__ __forceinline__ int few_place(int i) { return W == FEW_FP4_F16 ? (i & 3) * 2 + (i >> 2) : i; }
-__device__ __forceinline__ uint32_t f16x2_sat(float lo, float hi) {          // NaN stays NaN
-  uint32_t r;
-  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 
 // ------------------------------------------------------------------------------- ring of copies
 // Warps 0 .. 7 multiply, the others copy.  All waits are bounded; after a failed one every warp leaves its loop.
@@ -296,15 +298,16 @@ struct FewBefore {
   uint32_t mask[FEW_EXPERTS];        // tokens that meet an expert
 };
 // .. and behind the ring
-struct FewShared {
+struct alignas(16) FewShared {
   FewBars bars;
   float4 teams[2][4][64];             // [item][warp][half of its rows, lane] sums of the second team
   uint32_t top[FEW_TOKENS];          // bits of the rows' largest magnitudes
+  alignas(16) uint32_t item_top[2][4][4];        // [turn][pair of tokens][warp]: exponents of the largest of an item's activations
   FewPlan plan;
 };
 static_assert(sizeof(FewShared) % 16 == 0, "16-byte accesses to what follows");
 
-// Power of two that brings a row's largest magnitude (its bits) to 2^14 .. 2^15
+// Power of two that brings a largest magnitude (its bits) to 2^14 .. 2^15; none for one that is no number
 __device__ __forceinline__ int few_shift(uint32_t top) { return top >= 0x7f800000u ? 0 : min(14 - (int(top >> 23) - 127), 126); }
 // A float as an unsigned number of the same order; 0: not a number.
 __device__ __forceinline__ uint32_t few_key(float v) {
@@ -513,9 +516,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
   const int item0 = int(unsigned(items) * cluster / clusters), mine = int(unsigned(items) * (cluster + 1) / clusters) - item0;
   const unsigned all_steps = unsigned(mine * steps);
   const int lo = int(all_steps * rank / FEW_CLUSTER), hi = int(all_steps * (rank + 1) / FEW_CLUSTER);
-  // Activations of 16 features x 2 tokens a lane: acc[m] the sums of features m * 8 + g of the warp's 16 (gate, gate, up, up)
+  // Activations of 16 features x 2 tokens a lane: acc[m] the sums of features m * 8 + g of the warp's 16 (gate, gate, up, up).  For the first four warps together.
+  int turn = 0;
   auto finish = [&](int item, const float (&acc)[2][4]) {
     const int d = item / tiles, f0 = (item - d * tiles) * 64 + (warp & 3) * 16;
+    float h[2][2];                                       // [feature][token]
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
       const long long row = (long long)sh.plan.expert[d] * 2 * p.I + (f0 >> 6) * 128 + (f0 & 63) + m * 8 + g;
@@ -523,6 +528,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int t = q * 2 + j, slot = sh.plan.slot[d][t];
+        h[m][j] = 0.f;
         if (slot == 255) continue;
         const float s = W == FEW_FP4_F16 ? __uint_as_float(uint32_t(127 - few_shift(sh.top[t])) << 23) * Tile::SCALE : 1.f;
         float gate = fmaf(acc[m][j], s, bg), up = fmaf(acc[m][2 + j], s, bu), v = gate;
@@ -534,11 +540,42 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
           v = p.alpha * gate;
           up += 1.f;
         }
-        const int pair = t * p.top + slot;
-        v = gate / (1.f + expf(-v)) * up * sh.plan.share[pair];
-        p.h[(long long)pair * p.I + f0 + m * 8 + few_place<W>(g)] = uint16_t(W == FEW_FP4_F16 ? f16x2_sat(v, 0.f) : pack_bf16x2(v, 0.f));
+        h[m][j] = gate / (1.f + expf(-v)) * up * sh.plan.share[t * p.top + slot];
       }
     }
+    float scale[2] = {1.f, 1.f};
+    if (W == FEW_FP4_F16) {
+      // the largest of the item's 64 features, per token (its exponent, two tokens in a word): over the lanes of the warp that share the token, then over the four
+      // warps.  Two buffers: a warp is at most one item ahead of the others
+      __syncwarp();
+      auto exponent = [&](int j) { return max(__float_as_uint(h[0][j]) & 0x7fffffffu, __float_as_uint(h[1][j]) & 0x7fffffffu) >> 23; };
+      uint32_t top = exponent(0) | exponent(1) << 16;
+#pragma unroll
+      for (int o = 4; o < 32; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+      uint32_t (&all)[4][4] = sh.item_top[turn & 1];
+      ++turn;
+      if (g == 0) all[q][warp & 3] = top;
+      __syncwarp();
+      asm volatile("bar.sync 2, 128;" ::: "memory");
+      const uint4 w = *reinterpret_cast<const uint4*>(all[q]);
+      top = __vmaxu2(__vmaxu2(w.x, w.y), __vmaxu2(w.z, w.w));
+      float undo[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int shift = few_shift((top >> (16 * j) & 0xffffu) << 23);
+        scale[j] = __uint_as_float(uint32_t(127 + shift) << 23);
+        undo[j] = __uint_as_float(uint32_t(127 - shift) << 23) * Tile::SCALE;
+      }
+      if (warp == 0 && g == 0) *reinterpret_cast<float2*>(p.h_scale + ((long long)d * tiles + (f0 >> 6)) * FEW_TOKENS + q * 2) = make_float2(undo[0], undo[1]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int t = q * 2 + j, slot = sh.plan.slot[d][t];
+        if (slot == 255) continue;
+        p.h[(long long)(t * p.top + slot) * p.I + f0 + m * 8 + few_place<W>(g)] = uint16_t(W == FEW_FP4_F16 ? pack_f16x2(h[m][j] * scale[j], 0.f) : pack_bf16x2(h[m][j], 0.f));
+      }
   };
   const int last_item = hi > lo ? (hi - 1) / steps : 0;
   const bool open_end = hi > lo && hi % steps != 0 && last_item * steps >= lo;        // began here, ends elsewhere: finished below
@@ -653,7 +690,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
 template <int W>
 __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewArgs p) {
   using Tile = FewTile<W, FEW_DOWN_ROWS>;
-  constexpr int H_LD = Tile::CHUNKS * 128 + 64, H_OFF = Tile::CHUNKS * Tile::BYTES, STAGE = (H_OFF + FEW_TOKENS * H_LD + 1023) / 1024 * 1024;
+  constexpr bool SCALED = W == FEW_FP4_F16;            // a stage: weights, the tokens' activations, and (fp16 form) these's scales [step][token]
+  constexpr int H_LD = Tile::CHUNKS * 128 + 64, H_OFF = Tile::CHUNKS * Tile::BYTES, S_OFF = H_OFF + FEW_TOKENS * H_LD,
+                STAGE = (S_OFF + (SCALED ? Tile::CHUNKS * FEW_TOKENS * 4 : 0) + 1023) / 1024 * 1024;
   constexpr int STAGES = Tile::ring(FEW_DOWN_RING, STAGE), TEAMS = Tile::TEAMS;
   static_assert(STAGES >= TEAMS, "a place for every team");
   extern __shared__ uint8_t smem_raw[];
@@ -716,6 +755,15 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
     const int piece = lane & 15;                         // a half of the warp takes a token at a time, 16 bytes a lane
     const uint16_t* from[PAIRS] = {};                    // every second one of the tokens that meet expert `now`: its activations, and its place in a stage
     int place[PAIRS] = {}, pairs = 0, now = -1;
+    // What is small goes by pieces of 16 bytes, one a lane: scales of the weights' half records, then (fp16 form) the activations'.  A lane's piece is of step `of`.
+    constexpr bool HALVES = Tile::COPIED < Tile::BYTES;
+    constexpr int FIRST = HALVES ? Tile::CHUNKS * Tile::EACH : 0, LAST = FIRST + (SCALED ? Tile::CHUNKS * 2 : 0);
+    static_assert(LAST <= 32, "a piece a lane");
+    const bool weights = lane < FIRST;
+    const int of = lane >= LAST ? Tile::CHUNKS : weights ? lane / Tile::EACH : (lane - FIRST) >> 1;
+    const int small_to = weights ? of * Tile::BYTES + Tile::scales_in_step(lane % Tile::EACH) : S_OFF + (lane - FIRST) * 16;
+    const long long record = (long long)((p.H + 127) >> 7) * FP4_RECORD_BYTES, small_step = Tile::CHUNKS * (weights ? record : FEW_TOKENS * 4);
+    const uint8_t* small = nullptr;
     for (int i = lo; i < hi; ++i) {
       if (d != now) {
         now = d;
@@ -730,12 +778,20 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
           place[u] = t < 0 ? -1 : H_OFF + t * H_LD + piece * 16;
           if (t >= 0) from[u] = p.h + (long long)(t * p.top + plan.slot[d][t]) * p.I + piece * 8;
         }
+        if (LAST > 0) {
+          const uint8_t* tile = static_cast<const uint8_t*>(p.down) + (n0 >> 7) * FP4_RECORD_BYTES + Tile::scales_in_record(n0, lane % Tile::EACH);
+          small = weights ? tile + ((long long)plan.expert[d] * chunks + c + of) * record
+                          : reinterpret_cast<const uint8_t*>(p.h_scale + ((long long)d * chunks + c + of) * FEW_TOKENS) + (lane & 1) * 16;
+        }
       }
       ok = r.wait_empty(bars, p.status);
       if (!ok) break;
       const int n = min(Tile::CHUNKS, chunks - c);
       uint8_t* st = ring + r.s * STAGE;
-      if constexpr (Tile::COPIED < Tile::BYTES) Tile::copy_scales(st, p.down, plan.expert[d], n0, c, n, p.H, p.I, lane);
+      if (LAST > 0) {
+        if (of < n) cp_async16(st + small_to, small, true);
+        small += small_step;
+      }
 #pragma unroll
       for (int u = 0; u < PAIRS; ++u) {
         if (u >= pairs) break;
@@ -751,7 +807,8 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
   } else {
     float acc[2][4] = {};
     FewReader<STAGE, TEAMS> r(&bars, ring, STAGES, team);
-    const uint32_t place = Tile::place(r0, g, q), scales = Tile::scales(r0), hs = H_OFF + g * H_LD + q * 16;
+    const uint32_t place = Tile::place(r0, g, q), scales = Tile::scales(r0), hs = H_OFF + g * H_LD + q * 16, ss = S_OFF + q * 8;
+    auto scaling = [](const uint2& v) { return make_float2(__uint_as_float(v.x), __uint_as_float(v.y)); };
     auto masked = [](const uint4& v, uint32_t m) { return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m); };
     int i = lo + team;                                   // this team's next step
     for (int from = lo; from < hi; ++d) {
@@ -761,11 +818,11 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
         if (ok && (ok = r.wait(p.status))) {
           const uint32_t x = r.data + hs;
           uint4 b[2] = {masked(lds128<0>(x), meets), masked(lds128<64>(x), meets)};
-          Tile::mma(acc, r.data + place, r.data + scales, b);
+          Tile::template mma<SCALED>(acc, r.data + place, r.data + scales, b, scaling(SCALED ? lds64<0>(r.data + ss) : make_uint2(0u, 0u)));
           if ((i - begin) * Tile::CHUNKS + 1 < chunks) {
             b[0] = masked(lds128<128>(x), meets);
             b[1] = masked(lds128<192>(x), meets);
-            Tile::mma(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b);
+            Tile::template mma<SCALED>(acc, r.data + Tile::BYTES + place, r.data + Tile::BYTES + scales, b, scaling(SCALED ? lds64<FEW_TOKENS * 4>(r.data + ss) : make_uint2(0u, 0u)));
           }
           r.release(lane, acc);
         }
@@ -800,7 +857,7 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
     if (!output(i, n, t)) continue;
     float v = 0.f;
     for (int s = 0; s < splits * TEAMS; ++s) v += red[s * per + i];
-    p.out[(long long)t * p.H + n] = f2bf(fmaf(v, Tile::SCALE, bias[k]));
+    p.out[(long long)t * p.H + n] = f2bf(v + bias[k]);
   }
 }
 
@@ -873,7 +930,7 @@ static int LaunchFew(FewArgs p, int sm_count, cudaStream_t stream) {
 using namespace ogb;
 
 OGB_API long long ogb_moe_few_scratch_bytes(int T, int top, int I) {
-  return T < 1 || T > FEW_TOKENS || top < 1 || top > FEW_TOP || I < 1 ? -1 : (long long)sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL + (long long)T * top * I * 2;
+  return T < 1 || T > FEW_TOKENS || top < 1 || top > FEW_TOP || I < 1 ? -1 : (long long)sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL + (long long)T * top * (I * 2LL + I / 64 * (FEW_TOKENS * 4LL));
 }
 
 OGB_API int ogb_moe_few_takes(int T, int H, int I, int E, int top) {
@@ -890,7 +947,8 @@ OGB_API int ogb_moe_few_tokens(const void* x, long long ldx, const void* router,
   FewArgs p{static_cast<const __nv_bfloat16*>(x), ldx, static_cast<const __nv_bfloat16*>(router), static_cast<const __nv_bfloat16*>(router_b), gate_up,
             static_cast<const __nv_bfloat16*>(gate_up_b), down, static_cast<const __nv_bfloat16*>(down_b), static_cast<__nv_bfloat16*>(out), T, H, I, E, top,
             rule, act, alpha, limit, static_cast<FewPlan*>(scratch), reinterpret_cast<float4*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan)),
-            reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL), 0, 0, 0, status};
+            reinterpret_cast<uint16_t*>(static_cast<uint8_t*>(scratch) + sizeof(FewPlan) + FEW_MAX_CTAS * 4096LL), nullptr, 0, 0, 0, status};
+  p.h_scale = reinterpret_cast<float*>(p.h + (long long)T * top * I);
   if ((long long)E * 2 * I > 0x7fffffff || (long long)E * H > 0x7fffffff || (long long)min(E, T * top) * I * H > 1LL << 37) return -5;   // (32-bit counts of steps)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (weights == FEW_BF16) return LaunchFew<FEW_BF16>(p, sm_count, s);

@@ -992,7 +992,8 @@ def moe_few_tokens(x, router_w, router_b, gate_up_w, gate_up_b, down_w, down_b, 
     x [T, H] bf16, 1 <= T <= 8; router_w [E, H] and router_b [E] (or None) bf16; gate_up_w [E, 2I, H] in interleave_experts_gate_up's order and
     down_w [E, H, I]: bf16, or packed MXFP4 (Fp4Experts, both in the same form); gate_up_b [E, 2I] (in the same order) and down_b [E, H] bf16 or None.
     weights "selected": softmax over the chosen logits; "all": over all; "renormed": over all, then over the chosen (the same numbers as "selected").
-    act "silu": silu(gate) * up; "clamped": g sigmoid(alpha g) (u + 1), where limit > 0 with gate <= limit and |up| <= limit.  Returns [T, H] bf16."""
+    act "silu": silu(gate) * up; "clamped": g sigmoid(alpha g) (u + 1), where limit > 0 with gate <= limit and |up| <= limit.  Returns [T, H] bf16.
+    On CUDA devices the activations go from one product to the other in 16 bits (relative to their own size, or the largest of 64 neighbours)."""
     if weights not in _FEW_RULES or act not in _FEW_ACTS:
         raise ValueError(f"moe_few_tokens has no routing weights {weights!r} with the activation {act!r}")
     if x.dim() != 2 or not 1 <= x.shape[0] <= MOE_FEW_TOKENS:

@@ -185,3 +185,64 @@ def test_many_turns_of_the_rings_repeat(kind):
     torch.cuda.synchronize()
     assert int(differs) == 0
     ops.check_kernel_status()
+
+
+def fixed_choice(p, E):
+    """The router replaced by logits that do not go by the rows."""
+    p["router_w"] = torch.zeros_like(p["router_w"])
+    p["router_b"] = (torch.arange(E) % 5).to(torch.bfloat16).to(DEV)
+    return p
+
+
+def below(p, w, act):
+    """What the activations' 16 bits may lose below the normal numbers of fp16: with the largest of 64 neighbours at 2^14 or more, half a step of 2^-24 is 2^-39 of it."""
+    a = p["x"].double().abs()
+    most = torch.zeros(a.shape[0], 1, dtype=torch.float64, device=DEV)
+    for e in range(w["down"].shape[0]):
+        g, u = (a @ w["gate_up"][e].double().abs().T).chunk(2, dim=1)
+        most = torch.maximum(most, (g * (u + (act == "clamped"))).amax(1, keepdim=True) * w["down"][e].double().abs().sum(1).max())
+    return 2.0 ** -39 * most
+
+
+@pytest.mark.parametrize("act,limit", [("silu", 0.0), ("clamped", 1.5), ("clamped", 0.0)])
+@pytest.mark.parametrize("size", [-14, -8, 0, 8])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_any_size(kind, size, act, limit):
+    """Activations far below and above the range of 16-bit floats: every error is relative to what is added up, whatever its size."""
+    T, E, H, I = 5, 8, 1024, 320
+    p, w = layer(T, E, H, I, kind, False, seed=size + 20)
+    fixed_choice(p, E)
+    p["x"] = p["x"] * 2.0 ** size
+    p["x"][1] *= 2.0 ** -6                             # not all tokens of one size
+    args = dict(top=3, weights="selected", act=act, alpha=1.702 if act == "clamped" else 1.0, limit=limit)
+    got = ops.moe_few_tokens(**p, **args).double()
+    want, tol = exact(p, w, **args)
+    tol = tol - 1e-6 + below(p, w, act)
+    worst = float(((got - want).abs() / tol).max())
+    assert worst <= 1, f"off by {worst:.3g} times what the roundings allow"
+    assert float((got - want).norm() / want.norm()) < 2.0 ** -7          # (and as a whole: half a step of bf16 twice)
+    ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("act", ["silu", "clamped"])
+def test_infinities_are_not_cut_off(kind, act):
+    p, _ = layer(6, 8, 256, 128, kind, False)
+    fixed_choice(p, 8)
+    args = dict(top=2, weights="renormed", act=act, alpha=1.702 if act == "clamped" else 1.0, limit=0.0)
+    ref = ops.moe_few_tokens(**p, **args)
+    p["x"] = p["x"].clone()
+    p["x"][2, 5], p["x"][4, 0] = math.nan, math.inf
+    got = ops.moe_few_tokens(**p, **args)
+    keep = [0, 1, 3, 5]
+    assert torch.equal(got[keep], ref[keep]) and bool(torch.isnan(got[2]).all()) and not bool(torch.isfinite(got[4]).any())
+
+
+@pytest.mark.parametrize("weights", ["selected", "all"])
+def test_masked_experts(weights):
+    """Router biases of minus infinity: such experts are the last to be chosen, and count nothing."""
+    p, w = layer(3, 16, 128, 64, "bf16", True)
+    p["router_b"][3:] = -math.inf
+    args = dict(top=5, weights=weights, act="silu", alpha=1.0, limit=0.0)
+    want, tol = exact(p, w, **args)
+    assert bool(((ops.moe_few_tokens(**p, **args).double() - want).abs() <= tol).all())
