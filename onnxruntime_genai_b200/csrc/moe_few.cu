@@ -35,7 +35,7 @@ namespace ogb {
 template <int N> struct Int { static constexpr int value = N; };
 enum FewWeights : int { FEW_BF16 = 0, FEW_FP4_F16 = 1, FEW_FP4_BF16 = 2 };   // packed: the records of gemm_fp4.cu in their two forms
 constexpr int FEW_TOKENS = 8, FEW_TOP = 32, FEW_EXPERTS = 1024, FEW_MET = FEW_TOKENS * FEW_TOP;
-constexpr int FEW_CLUSTER = 8;
+constexpr int FEW_CLUSTER = 8, FEW_AGAIN = 0x8000;
 constexpr int FEW_THREADS = 288, FEW_DOWN_THREADS = 320, FEW_STAGES = 16;
 constexpr size_t FEW_SMEM_TWO = 113 * 1024, FEW_SMEM_ONE = 227 * 1024;          // shared memory of a CTA, with two or one on an SM
 constexpr int FEW_DOWN_ROWS = 64, FEW_DOWN_RING = 96 * 1024, FEW_OUT = FEW_DOWN_ROWS * FEW_TOKENS;
@@ -47,7 +47,7 @@ struct alignas(16) FewPlan {
   int met, unused[3];                       // experts that any token meets, in ascending order
   uint16_t expert[FEW_MET];
   uint8_t slot[FEW_MET][FEW_TOKENS];        // which choice of the token the expert is; 255: none
-  uint16_t ids[FEW_TOKENS * FEW_TOP];       // [token][choice]
+  uint16_t ids[FEW_TOKENS * FEW_TOP];       // [token][choice]; FEW_AGAIN: expert 0 again
   float share[FEW_TOKENS * FEW_TOP];
 };
 static_assert(sizeof(FewPlan) % 16 == 0, "h follows the plan");
@@ -314,8 +314,8 @@ __device__ __forceinline__ uint32_t few_key(float v) {
   const uint32_t u = __float_as_uint(v);
   return v != v ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// Choice of `top` experts for a token by one warp: the largest logits, the lowest index among equal ones; a token whose logits are not numbers takes
-// expert 0.  A lane holds every 32nd expert, up to 32 R, and looks for its best one anew only when that was taken.
+// Choice of `top` experts for a token by one warp: the largest logits, the lowest index among equal ones; where logits are not numbers, expert 0 stands for
+// what is missing (several times then), and all shares are no numbers.  A lane holds every 32nd expert, up to 32 R, and looks for its best one anew only when that was taken.
 template <int R>
 __device__ __forceinline__ void few_choose(const float* row, int E, int top, int rule, int lane, int& id, float& share) {
   uint32_t key[R];                   // 0: nothing to choose
@@ -478,8 +478,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     if (p.E <= 128) few_choose<4>(row, p.E, p.top, p.rule, lane, id, share);
     else if (p.E <= 256) few_choose<8>(row, p.E, p.top, p.rule, lane, id, share);
     else few_choose<32>(row, p.E, p.top, p.rule, lane, id, share);
+    // expert 0 may stand there several times: the first counts, so that all clusters look for its activations in the same place
+    const uint32_t zeros = __ballot_sync(0xffffffffu, id == 0);
+    const bool again = id == 0 && (zeros & ((1u << lane) - 1)) != 0;
     if (lane < p.top) {
-      sh.plan.ids[warp * p.top + lane] = uint16_t(id);
+      sh.plan.ids[warp * p.top + lane] = uint16_t(again ? FEW_AGAIN : id);
       sh.plan.share[warp * p.top + lane] = share;
       atomicOr(&pre.mask[id], 1u << warp);
     }
@@ -500,7 +503,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) few_gate_up_kernel(const __gri
     }
     if (lane == 0) sh.plan.met = n;
     __syncwarp();
-    for (int i = lane; i < p.T * p.top; i += 32) sh.plan.slot[pre.mask[sh.plan.ids[i]]][i / p.top] = uint8_t(i % p.top);
+    for (int i = lane; i < p.T * p.top; i += 32)
+      if (const int id = sh.plan.ids[i]; id < FEW_AGAIN) sh.plan.slot[pre.mask[id]][i / p.top] = uint8_t(i % p.top);
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // copies take the place of what stood in the ring's
   __syncthreads();
@@ -726,7 +730,7 @@ __global__ void __launch_bounds__(FEW_DOWN_THREADS, 2) few_down_kernel(const __g
     for (int k = 0; k < 2; ++k) {
       int n, t;
       if (output(int(threadIdx.x) + k * FEW_DOWN_THREADS, n, t))
-        for (int j = 0; j < p.top; ++j) bias[k] += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)plan.ids[t * p.top + j] * p.H + n]);
+        for (int j = 0; j < p.top; ++j) bias[k] += plan.share[t * p.top + j] * bf2f(p.down_b[(long long)(plan.ids[t * p.top + j] & (FEW_AGAIN - 1)) * p.H + n]);
     }
   }
   bool ok = true;

@@ -246,3 +246,23 @@ def test_masked_experts(weights):
     args = dict(top=5, weights=weights, act="silu", alpha=1.0, limit=0.0)
     want, tol = exact(p, w, **args)
     assert bool(((ops.moe_few_tokens(**p, **args).double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_tokens_whose_logits_are_no_numbers(kind):
+    """All logits of a token, or some, are NaN: the choice is short of experts.  Such a token's result is NaN every time, the others' as without it."""
+    p, _ = layer(8, 16, 256, 1024, kind, False)
+    args = dict(top=4, weights="selected", act="silu")
+    ref = ops.moe_few_tokens(**p, **args)
+    p["x"] = p["x"].clone()
+    p["x"][1], p["x"][6] = math.nan, math.nan
+    for _ in range(50):
+        junk = torch.ones(1 << 22, dtype=torch.bfloat16, device=DEV)        # what the call's scratch may find in its memory are numbers
+        del junk
+        got = ops.moe_few_tokens(**p, **args)
+        keep = [0, 2, 3, 4, 5, 7]
+        assert torch.equal(got[keep], ref[keep]) and bool(torch.isnan(got[[1, 6]]).all())
+    p["x"] = torch.where(torch.isnan(p["x"]), torch.ones_like(p["x"]), p["x"])
+    fixed_choice(p, 16)
+    p["router_b"][2:] = math.nan                       # two experts are left to choose four from
+    assert bool(torch.isnan(ops.moe_few_tokens(**p, **args)).all())
