@@ -71,6 +71,7 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
   }
   if (ROWS && threadIdx.x >= 64 && threadIdx.x < 64 + FP4_OWN_ROWS) s_top[threadIdx.x - 64] = 0;
   if (warp == 1) { tmem_alloc(tmem_slot, Cfg::COLS); tmem_relinquish(); }
+  __syncwarp();                                             // (lanes may be apart behind the branches above: the arrival wants whole warps)
   if (p.splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");         // sums are sent to CTAs that run
   tc_fence_before();
   __syncthreads();

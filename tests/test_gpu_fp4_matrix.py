@@ -265,3 +265,18 @@ def test_offsets_beyond_32_bits():
     xq, wq = ops.quantize_fp4(x[-5:], "mxfp4").dequantize().double(), w.dequantize().double()
     close(y, xq @ wq.T, xq.abs() @ wq.abs().T, 256)
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("T,given", [(1, False), (2, False), (2, True), (20, True), (60, True)])
+def test_parts_of_k_in_clusters_repeat(T, given):
+    """Products whose parts of k meet in a cluster, a hundred in a row: the same sums every time."""
+    x, w = rows_of("normal", T, 4096, torch.bfloat16).to(DEV), weight(640, 4096, "nvfp4")
+    rows = ops.quantize_fp4(x) if given else x
+    first = ops.linear(rows, w, out_fp32=True)
+    xq, wq = ops.quantize_fp4(x).dequantize().double(), w.dequantize().double()
+    close(first, xq @ wq.T, xq.abs() @ wq.abs().T, 4096)
+    differs = torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(100):
+        differs += (ops.linear(rows, w, out_fp32=True) != first).any()
+    assert int(differs) == 0
+    ops.check_kernel_status()
