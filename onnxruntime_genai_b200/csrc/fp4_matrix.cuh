@@ -53,6 +53,12 @@ __host__ __device__ inline long long fp4_scale_at(const Fp4View& v, int form, in
   return (((long long)kb * (v.padded >> 7) + (r >> 7)) * fp4_steps(form) + step) * FP4_SCALE_STEP + (r & 31) * 16 + ((r & 127) >> 5) * 4 + b;
 }
 
+__device__ __forceinline__ float reciprocal(float v) {      // within a last place or two, of a normal number
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Codes to numbers, by their fields.
 __device__ __forceinline__ float fp4_value(uint32_t code) {     // e2m1
   const uint32_t m = code & 7u;

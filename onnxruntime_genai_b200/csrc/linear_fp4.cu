@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(192, 3) linear_fp4_kernel(const Fp4LinearArgs 
         for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], scale * ws[j], wb[j]);
         if (p.pair) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = silu(v[j]) * fmaf(u[j], scale * us[j], ub[j]);
+          for (int j = 0; j < 8; ++j) v[j] = fp4_silu(v[j]) * fmaf(u[j], scale * us[j], ub[j]);
         }
         fp4_store8(p, m, col, v);
       }

@@ -56,6 +56,9 @@ __device__ __forceinline__ void fp4_mma(uint32_t d, uint64_t da, uint64_t db, ui
 }
 
 // ------------------------------------------------------------------------------- results
+// v / (1 + exp(-v)) by a reciprocal, a few 2^-23 off; below some -87, where the result is under 2^-119, zero.  (With an IEEE division 8192 gated tokens of
+// 4096 -> 2 x 14336 take 501 us instead of 409.)
+__device__ __forceinline__ float fp4_silu(float v) { return v * reciprocal(1.f + __expf(-v)); }
 // Eight columns of token row m: residual and store.
 __device__ __forceinline__ void fp4_store8(const Fp4LinearArgs& p, int m, int col, float (&v)[8]) {
   const int n = min(8, p.n_out - col);

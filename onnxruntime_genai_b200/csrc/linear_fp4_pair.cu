@@ -218,7 +218,7 @@ linear_fp4_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
           float v[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
           const float u[8] = {h0.x, h0.y, h0.z, h0.w, h1.x, h1.y, h1.z, h1.w};
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[q] = silu(fmaf(v[q], sc * ws[q], wb[q])) * fmaf(u[q], sc * us[q], ub[q]);
+          for (int q = 0; q < 8; ++q) v[q] = fp4_silu(fmaf(v[q], sc * ws[q], wb[q])) * fmaf(u[q], sc * us[q], ub[q]);
           if (c0 + tok < rows && col < p.n_out) fp4_store8(p, x.row0 + c0 + tok, col, v);
         } else {
           __syncwarp();

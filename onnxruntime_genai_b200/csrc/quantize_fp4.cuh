@@ -29,11 +29,6 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(code)));
   return __half2float(__ushort_as_half(uint16_t(h)));
 }
-__device__ __forceinline__ float reciprocal(float v) {      // within a last place or two, of a normal number
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // eight numbers to eight codes, the first in the lowest four bits: to nearest, ties to the even code, at most 6
 __device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
   uint32_t r;

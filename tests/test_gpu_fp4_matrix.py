@@ -280,3 +280,18 @@ def test_parts_of_k_in_clusters_repeat(T, given):
         differs += (ops.linear(rows, w, out_fp32=True) != first).any()
     assert int(differs) == 0
     ops.check_kernel_status()
+
+
+@pytest.mark.parametrize("T", [3, 40, 70, 200])
+def test_results_near_the_smallest_normal_numbers(T):
+    """Scales whose product is below the normal numbers, and results around their border: the same rules whichever kernel takes the rows."""
+    N, K = 128, 256
+    small = weight(N, K, "nvfp4")
+    c = small.codes()
+    w = ops.Fp4Matrix.from_codes(c[:, 0::2] | c[:, 1::2] << 4, small.scales(), small.row_scales() * 2.0 ** -58)
+    x = (rows_of("normal", T, K, torch.float32) * 2.0 ** -66).to(DEV)
+    xq, wq = ops.quantize_fp4(x).dequantize().double(), w.dequantize().double()
+    want, size = xq @ wq.T, xq.abs() @ wq.abs().T
+    assert float(want.abs().max()) > 2.0 ** -126
+    # the bounds of `close`, and half a step of the subnormal numbers, 2^-150, for the result
+    assert bool(((ops.linear(x, w, out_fp32=True).double() - want).abs() <= (K / 16 + 8) * 2.0 ** -23 * size + 2.0 ** -150).all())
