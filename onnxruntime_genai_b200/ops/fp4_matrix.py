@@ -16,6 +16,7 @@ import torch
 
 FORMS = {"nvfp4": 0, "mxfp4": 1}
 BLOCK = {"nvfp4": 16, "mxfp4": 32}
+LARGEST = {"nvfp4": 0x7e, "mxfp4": 0xfe}   # bytes of block scales: 0x7f and 0xff are not numbers, and e4m3 scales have no sign
 KB = 256                                   # k values of a k-block
 E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
 
@@ -91,7 +92,7 @@ class Fp4Matrix:
     def from_codes(codes: torch.Tensor, scales: torch.Tensor, scale: Optional[torch.Tensor] = None, form: str = "nvfp4", device=None,
                    interleaved: bool = False) -> "Fp4Matrix":
         """codes uint8 [N, K/2] (the even k in the low half of a byte); scales [N, K/block]: bytes, or float8_e4m3fn; scale: fp32, one number, one per row
-        ([N]), or None (1).  The layout is made where `codes` lives and moved to `device`.  interleaved: the rows are in interleave_gate_up's order."""
+        ([N]), or None (1).  Scales that are not numbers, or negative, are refused.  The layout is made where `codes` lives and moved to `device`.  interleaved: the rows are in interleave_gate_up's order."""
         if codes.dim() != 2 or codes.dtype != torch.uint8:
             raise ValueError("codes are uint8 [N, K/2]")
         N, K = codes.shape[0], codes.shape[1] * 2
@@ -100,6 +101,8 @@ class Fp4Matrix:
         scales = scales.view(torch.uint8) if scales.dtype != torch.uint8 else scales
         if scales.shape != (N, per):
             raise ValueError(f"block scales have the shape {tuple(scales.shape)}: {(N, per)} is wanted")
+        if bool((scales > LARGEST[form]).any()):
+            raise ValueError(f"a block scale of {int(scales.max()):#x}: {form} scales are numbers without a sign, bytes up to {LARGEST[form]:#x}")
         if scale is not None and scale.numel() not in (1, N):
             raise ValueError(f"{scale.numel()} scales for {N} rows")
         if interleaved and N % 128:

@@ -165,3 +165,18 @@ def test_launchers_refuse_on_the_host():
     linear = lambda T=4, N=128, K=64, form=0, pair=0, res=None, w=W: L.ogb_linear_fp4(A, 64, 0, W, T, w, N, K, form, C, N, 0, pair, None, res, N, 0, None, 148, None)
     assert linear(T=-1) == -1 and linear(N=0) == -1 and linear(K=40) == -1 and linear(form=2) == -1 and linear(w=W + 4) == -1
     assert linear(N=64, pair=1) == -1 and linear(pair=1, res=C) == -1 and linear(T=0) == 0
+
+
+def test_block_scales_that_are_no_numbers():
+    codes = torch.full((2, 32), 0x22, dtype=torch.uint8)
+    for form, good, bad in (("nvfp4", 0x7e, (0x7f, 0x80, 0xb8, 0xff)), ("mxfp4", 0xfe, (0xff,))):
+        scales = torch.full((2, 64 // fp4_matrix.BLOCK[form]), 0x30, dtype=torch.uint8)
+        scales[1, 1] = good
+        assert bool(torch.isfinite(ops.Fp4Matrix.from_codes(codes, scales, form=form).dequantize()).all())
+        for b in bad:
+            scales[1, 1] = b
+            with pytest.raises(ValueError, match="block scale"):
+                ops.Fp4Matrix.from_codes(codes, scales, form=form)
+            if form == "nvfp4":
+                with pytest.raises(ValueError, match="block scale"):
+                    ops.Fp4Matrix.from_codes(codes, scales.view(torch.float8_e4m3fn), form=form)
