@@ -385,15 +385,12 @@ def linear(x, w, bias=None, residual=None, out_fp32=False, out=None, splits=0, a
     splits: 0 leaves the kernel to the launcher; n > 0 asks for the one that cuts k in n parts, n < 0 for the one on pairs of SMs with -n token
     tiles where it can take the product (no reduction over ranks, no folded norm).
     w an Fp4Matrix: x (bf16 or fp32 rows, or an Fp4Matrix of the same form) is quantised to 4 bits too, and the block-scaled tensor-core product takes both
-    as they are; splits is not looked at, and `out` may be the residual, but must not overlap the rows."""
+    as they are; splits is not looked at, and `out` may be the residual, but must not overlap the rows.  Without out_fp32 results are bf16 on CUDA devices,
+    fp32 rows or not, and of the rows' type on the CPU."""
     if isinstance(w, Fp4Matrix):
         if all_reduce or reduce_scatter is not None:
             raise RuntimeError("products of 4-bit floating-point weights are not reduced over ranks")
-        if norm_eps > 0:
-            if isinstance(x, Fp4Matrix):
-                raise ValueError("a norm cannot be folded into rows that are quantised already")
-            x = rms_scale(x, norm_eps)
-        return _linear_fp4(x, w, bias, residual, out_fp32, out)
+        return _linear_fp4(_normed_rows(x, norm_eps), w, bias, residual, out_fp32, out)
     if isinstance(w, W4Weight):
         if norm_eps > 0:
             x = rms_scale(x, norm_eps)
@@ -471,6 +468,20 @@ def _dequantize_fp4(m: Fp4Matrix, dtype):
     out = torch.empty(m.rows, m.K, dtype=dtype, device=m.device)
     _call_on(m.data.get_device(), "ogb_dequantize_fp4", m.data.data_ptr(), m.rows, m.K, fp4_matrix.FORMS[m.form], out.data_ptr(), m.K, dtype == torch.float32)
     return out
+
+
+def _normed_rows(x, eps: float):
+    """Rows in front of a 4-bit product: as they are, or (eps > 0) over their root mean square, bf16 or fp32 as they came."""
+    if eps <= 0:
+        return x
+    if isinstance(x, Fp4Matrix):
+        raise ValueError("a norm cannot be folded into rows that are quantised already")
+    if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float32):          # (other types are refused by the product)
+        return rms_scale(x, eps) if not x.is_cuda else x
+    x = x.contiguous()
+    if x.dtype == torch.float32:
+        return norm_stream(x, torch.ones(x.shape[1], dtype=torch.float32, device=x.device), eps, dtype=torch.float32)
+    return rms_scale(x, eps)
 
 
 def _linear_fp4(x, w: Fp4Matrix, bias=None, residual=None, out_fp32=False, out=None, pair=False):
@@ -591,14 +602,12 @@ _PAIR_FLAGS = {"silu": 0, "relu": GEMM_PAIR_RELU, "gelu_tanh": GEMM_PAIR_GELU, "
 def gate_up_act(x, w, bias=None, act="silu", out=None, splits=0, interleaved=False, norm_eps=0.0):
     """act(x @ Wg.T) * (x @ Wu.T).  w is [2I, K]: stacked [Wg; Wu], or (interleaved=True) blocks of 64 gate
     rows + 64 up rows as produced by interleave_gate_up (the layout the fused kernel needs).  norm_eps, splits: as in `linear`.
-    w an Fp4Matrix: as in `linear`; its own `interleaved` tells the order of its rows."""
+    w an Fp4Matrix: as in `linear`; its own `interleaved` tells the order of its rows.  silu with interleaved rows is the epilogue of one product, from its fp32 sums;
+    else gate and up are rounded to the result's type before the activation, as those of other weights are where no epilogue pairs them."""
     if isinstance(w, Fp4Matrix):
-        if norm_eps > 0:
-            if isinstance(x, Fp4Matrix):
-                raise ValueError("a norm cannot be folded into rows that are quantised already")
-            x = rms_scale(x, norm_eps)
         if w.rows % 2:
             raise ValueError(f"{w.rows} gate and up rows")
+        x = _normed_rows(x, norm_eps)
         if act == "silu" and w.interleaved:
             return _linear_fp4(x, w, bias, None, False, out, pair=True)
         y = _linear_fp4(x, w, bias)

@@ -295,3 +295,20 @@ def test_results_near_the_smallest_normal_numbers(T):
     assert float(want.abs().max()) > 2.0 ** -126
     # the bounds of `close`, and half a step of the subnormal numbers, 2^-150, for the result
     assert bool(((ops.linear(x, w, out_fp32=True).double() - want).abs() <= (K / 16 + 8) * 2.0 ** -23 * size + 2.0 ** -150).all())
+
+
+def test_a_norm_in_front_of_rows_of_either_type_and_stride():
+    """norm_eps with fp32 rows, and with rows that do not lie together: the product of the normed rows."""
+    T, K = 5, 512
+    wide = rows_of("normal", T, K + 8, torch.float32).to(DEV) * 3.0
+    w, gated = weight(192, K, "nvfp4"), weight(256, K, "nvfp4", interleaved=True)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = wide.to(dtype)[:, 3:K + 3]
+        xd = x.double()
+        normed = xd * torch.rsqrt((xd * xd).mean(-1, keepdim=True) + 1e-5)
+        rows = ops._normed_rows(x, 1e-5)
+        # a sum of K squares, a root and a product in fp32, then the rows' type
+        assert rows.dtype == dtype and bool(((rows.double() - normed).abs() <= ((K + 8) * 2.0 ** -24 + (2.0 ** -8 if dtype == torch.bfloat16 else 0)) * normed.abs()).all())
+        assert torch.equal(ops.linear(x, w, norm_eps=1e-5), ops.linear(rows, w)) and torch.equal(ops.gate_up_act(x, gated, norm_eps=1e-5), ops.gate_up_act(rows, gated))
+    with pytest.raises(ValueError, match="bfloat16 or float32"):
+        ops.linear(wide.half()[:, :K], w, norm_eps=1e-5)
