@@ -1036,12 +1036,12 @@ class DecoderModel:
         return n
 
     def _all_tensors(self):
-        for t in (self.embed, self.final_norm_w, self.final_norm_b, self.lm_head_w, self.lm_head_b, self.cos, self.sin):
-            if t is not None:
-                yield t
+        """Every tensor of the weights, and those that packed weights lie in."""
         seen = set()
-        for lw in self.layers:
-            for v in vars(lw).values():
-                if isinstance(v, torch.Tensor) and id(v) not in seen:      # layers may share weights
-                    seen.add(id(v))
-                    yield v
+        fixed = (self.embed, self.final_norm_w, self.final_norm_b, self.lm_head_w, self.lm_head_b, self.cos, self.sin)
+        for v in (*fixed, *(v for lw in self.layers for v in vars(lw).values())):
+            if not isinstance(v, torch.Tensor):
+                v = v.data if isinstance(v, ops.Fp4Matrix) else getattr(v, "packed", None)
+            if isinstance(v, torch.Tensor) and id(v) not in seen:      # layers may share weights
+                seen.add(id(v))
+                yield v

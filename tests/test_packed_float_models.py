@@ -88,3 +88,13 @@ def test_layers_the_few_token_form_takes(monkeypatch):
     assert not moe._few_ok(lw, spec, x)
     lw.exp_shared, lw.shared_gate_up_w = False, torch.zeros(2, 2)
     assert not moe._few_ok(lw, spec, x)
+
+
+def test_bytes_of_packed_weights(tmp_path, monkeypatch):
+    arch = ArchConfig(**BASE)
+    export_model(copy.deepcopy(arch), str(tmp_path), "fp32", "cpu", state_dict=random_state_dict(arch, seed=1, std=0.1), linear_format="nvfp4")
+    expanded = og.Model(str(tmp_path)).decoder
+    monkeypatch.setenv("OGB_FP4_LINEAR", "1")
+    packed = og.Model(str(tmp_path)).decoder
+    pairs = [(packed.lm_head_w, expanded.lm_head_w)] + [(getattr(a, n), getattr(b, n)) for a, b in zip(packed.layers, expanded.layers) for n in ("qkv_w", "o_w", "gate_up_w", "down_w")]
+    assert packed.weight_bytes() - expanded.weight_bytes() == sum(p.data.numel() - 4 * e.numel() for p, e in pairs)
