@@ -197,3 +197,68 @@ def test_engine_with_packed_weights_and_experts(tmp_path, monkeypatch):
                 seen[id(r)].append(r.get_unseen_token())
     ops.check_kernel_status()
     assert all(0 < len(t) <= 12 and all(0 <= v < 1024 for v in t) for t in seen.values())
+
+
+def run_engine(engine, model, lengths, new):
+    rng = np.random.RandomState(3)
+    requests = []
+    for n in lengths:
+        gp = og.GeneratorParams(model)
+        gp.set_search_options(max_length=n + new, min_length=n + new)
+        r = og.Request(gp)
+        r.add_tokens(rng.randint(1, 1000, size=n).astype(np.int32))
+        engine.add_request(r)
+        requests.append(r)
+    seen = {id(r): [] for r in requests}
+    while engine.has_pending_requests():
+        r = engine.step()
+        if r is not None:
+            while r.has_unseen_tokens():
+                seen[id(r)].append(r.get_unseen_token())
+    ops.check_kernel_status()
+    return [seen[id(r)] for r in requests]
+
+
+@pytest.mark.parametrize("few", [False, True])
+def test_every_call_of_an_engine(few, tmp_path, monkeypatch):
+    """Prompts, mixed steps and padded batches of an engine: every product and expert layer against its definition on the rows it was given (padded rows may hold anything,
+    and are looked at only where they are numbers); and batches that need no padding give the same tokens from graphs as eagerly."""
+    from onnxruntime_genai_b200.engine.engine import ModelExecutor
+    arch = ArchConfig(vocab_size=1024, hidden_size=256, num_layers=2, num_heads=4, num_kv_heads=4, head_dim=64, intermediate_size=128, context_length=256,
+                      bos_token_id=0, eos_token_id=1023, pad_token_id=0, model_type="gptoss", num_experts=8, experts_per_token=2, attn_bias=True, o_bias=True,
+                      mlp_bias=True, attn_sinks=True, sliding_window=16, sliding_layers=[0])
+    d = str(tmp_path)
+    export_model(copy.deepcopy(arch), d, "int4", "cuda", state_dict=random_state_dict(arch, seed=8, std=0.05), linear_format="nvfp4", paged=True, block_size=16,
+                 num_blocks=256, max_batch_size=16)
+    monkeypatch.setenv("OGB_FP4_LINEAR", "1")
+    monkeypatch.setenv("OGB_ENGINE_RUN_AHEAD", "0")
+    monkeypatch.setenv("OGB_ENGINE_LOOKAHEAD", "0")
+    monkeypatch.setattr(moe, "_FEW", few)
+    model = og.Model(d)
+    lengths = (5, 70, 1, 9, 33, 2, 17, 8)
+    replayed = run_engine(og.Engine(model), model, lengths, 12)
+    assert all(len(t) == 12 for t in replayed)
+
+    def eager(self, bb, cb):
+        s = self._step_inputs(bb, bb, self.staging.table_cols, 1, cb * self.kv.block_size, ordered=self.order_attention)
+        logits = torch.empty(bb, 1024, dtype=torch.float32, device=DEV)
+        return type("Step", (), {"replay": lambda _: logits.copy_(self.decoder.forward(s, self.kv))})(), logits
+
+    calls = {"product": 0, "experts": 0}
+    product, experts = ops._linear_fp4, ops.moe_few_tokens
+
+    def near(got, want, tol, name):
+        calls[name] += 1
+        rows = torch.isfinite(want).all(-1)
+        assert bool(((got.double() - want).abs() <= tol)[rows].all()) and not bool(torch.isfinite(got[~rows].double()).all(-1).any()), f"{name} {calls[name]}"
+        return got
+
+    def products(x, w, bias=None, residual=None, out_fp32=False, out=None, pair=False):
+        want = exact_product(x, w, bias, residual, out_fp32, pair)
+        return near(product(x, w, bias, residual, out_fp32, out, pair), *want, "product")
+    monkeypatch.setattr(ModelExecutor, "_capture", eager)
+    assert run_engine(og.Engine(model), model, lengths, 12) == replayed
+    monkeypatch.setattr(ops, "_linear_fp4", products)
+    monkeypatch.setattr(ops, "moe_few_tokens", lambda *a: near(experts(*a), *exact_experts(*a), "experts"))
+    run_engine(og.Engine(model), model, lengths[:5], 6)                      # steps of one token a request are padded to eight
+    assert calls["product"] >= 5 * 6 and (calls["experts"] >= 2 * 5) == few
