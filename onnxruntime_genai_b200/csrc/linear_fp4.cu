@@ -314,8 +314,8 @@ static int fp4_splits(int N, int num_kb, int sm_count) { return max(1, min(min(8
 template <int FORM>
 static int LaunchLinear(const Fp4LinearArgs& p, int sm_count, cudaStream_t stream) {
   const int T = p.a.rows, bt = T <= 16 ? 16 : T <= 32 ? 32 : 64;
-  // (65 / 128 tokens, us here against pairs of SMs: 6144 x 4096 14.5 / 20.4 against 7.1 / 7.5, 28672 x 4096 14.5 / 17.6 against 12.2 / 13.7, 4096 x 14336 11.8 / 16.1
-  // against 14.5 / 14.7)
+  // (65 / 128 tokens, us with 128 token columns here, a form that was not kept, against pairs of SMs: 6144 x 4096 14.5 / 20.4 against 7.1 / 7.5, 28672 x 4096 14.5 / 17.6
+  // against 12.2 / 13.7; only few weight tiles with a long k were faster here, and by 65 tokens only: 4096 x 14336 11.8 / 16.1 against 14.5 / 14.7)
   if (T > 64) return LaunchPairLinearFp4(p, FORM, sm_count, stream);
   const int splits = fp4_splits(p.N, p.w.num_kb, sm_count);
   if (p.x) return p.x_fp32 ? LaunchFew<16, FORM, FP4_FP32>(p, splits, stream) : LaunchFew<16, FORM, FP4_BF16>(p, splits, stream);

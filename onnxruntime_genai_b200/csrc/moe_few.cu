@@ -16,8 +16,8 @@
 // of 7 tokens in 30 us instead of 40.
 //
 // Measured (us a layer, weights from memory; both kernels take 18 of them with hardly any weights: launches, the router, the choice, the first bytes, the sums):
-// 1 token, 4 of 32 mxfp4 experts of 2880: 28; 7 tokens of the same 87 (3.0 TB/s); 8 tokens, 8 of 128 of 1472: 111 (3.2); 1 token, 8 of 128 bf16 experts of 768: 26;
-// 8 tokens, 2 of 8 bf16 experts of 14336: 438 (5.8).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
+// 1 token, 4 of 32 mxfp4 experts of 2880: 28 (in their bf16 form 32); 7 tokens of the same 86 (3.0 TB/s; 115); 8 tokens, 8 of 128 of 1472: 109.5 (3.2); 1 token, 8 of 128
+// bf16 experts of 768: 26 to 28; 8 tokens, 2 of 8 bf16 experts of 14336: 438 to 454 on different cards (5.6 to 5.8).  With the products left out 7 mxfp4 tokens save 15 us of 98, with the activations' bulk copies left out 10.
 //
 // Roundings: the router's logits, all sums and the activation are fp32.  The activations times routing weights travel between the kernels in 16 bits (the
 // operand type of the second product): bf16, or, with packed experts in their fp16 form, fp16 after a scaling by a power of two per token, expert and 64 features

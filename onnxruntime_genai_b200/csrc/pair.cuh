@@ -34,8 +34,8 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
 // the first one: the text of the memory model does not order them.  What this rests on: the data concerned are the arriving CTA's own shared memory, whose
 // writers have each passed the proxy fence (which completes their stores) before their warp arrives, and its tensor memory, whose reads are complete after
 // tcgen05.wait; no cache lies between them and the tensor core that the arrival releases.  Arrivals of the scope of the cluster, all of them or relayed by one
-// warp of the second CTA, would be ordered by the text too and cost (us, none / all / relayed): int4 777 tokens, N 16384 77 / 115 / 107,
-// MXFP4 6000 rows of 32 experts, 5760 x 2880 178 / 277 / 266.
+// warp of the second CTA, would be ordered by the text too and cost (us, none / all / relayed): the int4 product of 777 tokens at the head of gemm_pair.cu
+// 77 / 115 / 107, MXFP4 6000 rows of 32 experts, 5760 x 2880 178 / 277 / 266.
 __device__ __forceinline__ void cluster_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
