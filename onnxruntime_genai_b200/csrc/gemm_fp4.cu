@@ -253,10 +253,6 @@ constexpr int FP4_STREAM_RES_BYTES = FP4_STREAM_TOKENS * GEMM_BLOCK_N * 4;
 constexpr int FP4_STREAM_FIXED_BYTES = FP4_STREAM_RING_BYTES + FP4_STREAM_RES_BYTES + 256;   // + barriers, abort flag
 constexpr int FP4_STREAM_SMEM_MAX = FP4_STREAM_FIXED_BYTES + FP4_STREAM_TOKENS * (FP4_STREAM_MAX_K * 2 + FP4_STREAM_XPAD);
 
-__device__ __forceinline__ void mma_m16n8k16_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __global__ void __launch_bounds__(FP4_STREAM_THREADS, 2)
 fp4_stream_grouped_kernel(const void* __restrict__ A_, int lda, const int* __restrict__ row_map, const uint8_t* __restrict__ wpacked,
                           int n_tiles_per_expert, int stage_rows, const GemmParams p) {

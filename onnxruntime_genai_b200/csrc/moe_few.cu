@@ -74,10 +74,6 @@ struct FewArgs {
 
 // ------------------------------------------------------------------------------- operands
 // (volatile: they are for whole warps, and must not be moved into a branch that some lanes take)
-__device__ __forceinline__ void few_mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void few_mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -168,7 +164,7 @@ struct FewTile {
           cvt_e2m1x8_f16(i ? (m ? q10.y : q00.y) : (m ? q10.x : q00.x), u);
           cvt_e2m1x8_f16(i ? (m ? q11.y : q01.y) : (m ? q11.x : q01.x), v);
           few_mma_f16_first(t[m][i], u[0], v[0], u[1], v[1], b[i].x, b[i].y);
-          few_mma_f16(t[m][i], u[2], v[2], u[3], v[3], b[i].z, b[i].w);
+          mma_m16n8k16_f16(t[m][i], u[2], v[2], u[3], v[3], b[i].z, b[i].w);
         }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
